@@ -15,7 +15,8 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, 'monoloco_amd', 'csrc')
 ASM_DIR = os.path.join(ROOT, 'monoloco_amd', 'lib', 'asm')
-FLAGS = ['-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '--offload-arch=gfx950', '-Wall', '-Wno-unused-function']   # = csrc/Makefile CXXFLAGS
+FLAGS = ['-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '--offload-arch=gfx950', '-Wall', '-Wno-unused-function',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']   # = csrc/Makefile CXXFLAGS
 
 
 def sources_mtime():
