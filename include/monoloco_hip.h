@@ -417,6 +417,55 @@ int ml_iou_matches_host(const double* boxes, int64_t m, int64_t ldb, const doubl
 int ml_xyz_from_distance_host(const float* d, int d_is_scalar, const float* centres, int64_t m, float* out);
 const char* ml_matching_last_error(void);
 
+/* ---- 8-bit residual block: quantisation, block-scaled product, root-mean-square norm, AdamW over many tensors ---------------- */
+/* The 8-bit format: OCP e4m3 codes in blocks of 128 values that share one scale, an e8m0 byte b = 2^(b - 127): the smallest power of two
+ * with which the block's largest magnitude fits into 448 (a block of zeros: 127; at least 1).  A block that holds a NaN or an infinity
+ * has scale 255 = NaN and NaN codes.  A block is 1 x 128 of a row (scales: (rows, ceil(cols / 128))) or 128 x 128 of a matrix ("tile":
+ * (ceil(rows / 128), ceil(cols / 128))); the last block of a row may be shorter.  No counterpart in the reference, whose layers are fp32.
+ * All sizes are element counts, all ld* row strides in elements; every operand's last axis is contiguous; pointers need the alignment of
+ * their element only (16-byte aligned rows take wider accesses).  Asynchronous on `stream`, nothing is allocated or kept: these calls may
+ * be captured into a graph (ml_adamw_step refuses: its step number is part of the launch).  Error text: ml_ops_last_error(). */
+#define ML_F32 0
+#define ML_BF16 1
+#define ML_F16 2
+/* x (m, n) -> codes q (m, n) + scales (1 x 128 blocks, or 128 x 128 with tile != 0) and / or, from the same read, the transposed matrix qt
+ * (n, m) in blocks of ITS rows (tile: the same tiles, transposed).  q or qt may be NULL, not both.  colsum_dev (ceil(m / 128), n) or NULL:
+ * fp32 sums of x over every 128 rows (ml_sum_rows joins them: the bias gradient of a linear layer). */
+int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t ldx, int tile, uint8_t* q_dev, int64_t ldq,
+                    uint8_t* scale_dev, int64_t lds, uint8_t* qt_dev, int64_t ldqt, uint8_t* scale_t_dev, int64_t ldst,
+                    float* colsum_dev, void* stream);
+/* c (m, n) = a (m, k) . b (n, k)^T [+ bias (n)] in fp32 accumulation, rounded once to c_dtype; a, b codes with scales per row block or
+ * per tile (a_tile, b_tile).  k = 0 gives the bias (or zeros).  16-bit results come from the 8-bit matrix instructions (1.5e-5 of the result's
+ * norm, far below their rounding), fp32 results from exact bf16 operands at half the rate (4e-8); there the values that the operands stand
+ * for have to lie in fp32's normal range (smaller ones count as 0). */
+int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
+                  const uint8_t* b_scale_dev, int64_t ldsb, int b_tile, const void* bias_dev, int bias_dtype, void* c_dev, int c_dtype,
+                  int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream);
+/* h = x [+ residual]; y = h / sqrt(mean(h^2) + eps) * w over rows of n.  x, residual, h, y of `dtype`; w (n) of `dtype` or fp32.  Exactly one
+ * of y_dev and q_dev (+ scale_dev: y as 1 x 128 blocks of codes) is written; h_dev may be NULL.  y and the row statistics come from h
+ * before its rounding to `dtype`. */
+int ml_rms_norm(const void* x_dev, int64_t ldx, const void* residual_dev, int64_t ldr, int dtype, const void* w_dev, int w_dtype, int64_t m,
+                int64_t n, float eps, void* h_dev, int64_t ldh, void* y_dev, int64_t ldy, uint8_t* q_dev, int64_t ldq, uint8_t* scale_dev,
+                int64_t lds, void* stream);
+/* Backward of ml_rms_norm from h (what it wrote): dx (m, n) = gradient of x and of the residual alike, [+ dh, the gradient that reaches h
+ * itself]; dw (n) of w_dtype.  work_dev: ml_rms_norm_backward_groups(m, n) * n floats.  Sums in a fixed order. */
+int64_t ml_rms_norm_backward_groups(int64_t m, int64_t n);
+int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int64_t ldh, const void* dh_dev, int64_t ldd, int dtype,
+                         const void* w_dev, int w_dtype, int64_t m, int64_t n, float eps, void* dx_dev, int64_t ldx, void* dw_dev,
+                         float* work_dev, void* stream);
+/* out (n) of `dtype` = sum over the rows of part (rows, n), fp32, in a fixed order. */
+int ml_sum_rows(const float* part_dev, int64_t rows, int64_t n, void* out_dev, int dtype, void* stream);
+/* One AdamW step, in place, over n_tensors contiguous tensors of one dtype that do not overlap (the reference's optimizer is torch's Adam,
+ * monoloco/train/trainer.py:128):  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+ * p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps).  Host arrays of device pointers; they may be reused as
+ * soon as the call returns.  scales == NULL: exp_avgs / exp_avg_sqs are fp32.  Otherwise they are e4m3 codes of m and of sqrt(v) in blocks of
+ * 128 along the flattened tensor, scales[i] holds ceil(numel / 128) bytes for m, then as many for sqrt(v), and both are rounded
+ * stochastically from (seed, step, i, element). */
+int ml_adamw_step(int n_tensors, const int64_t* numel, void* const* params, const void* const* grads, int dtype, void* const* exp_avgs,
+                  void* const* exp_avg_sqs, uint8_t* const* scales, int64_t step, double lr, double beta1, double beta2, double eps,
+                  double weight_decay, uint32_t seed, void* stream);
+const char* ml_ops_last_error(void);
+
 /* ---- measurement: per-launch timing of the dense (MFMA) kernel ----------------------- */
 /* After ml_loco_profile_begin, every dense-kernel launch made through this handle is bracketed by
  * a pair of HIP events recorded on the launch stream (up to max_launches launches).

@@ -31,6 +31,9 @@ ML_DEBUG_MID_SPLIT4 = 16384
 ML_DEBUG_MID_NODMA = 32768
 ML_FLAG_MERGE_W2W3 = 1
 ML_FLAG_HOST_ONLY = 256
+ML_F32 = 0
+ML_BF16 = 1
+ML_F16 = 2
 ML_OUT_STRIDE = 16
 ML_XYZDS_STRIDE = 5
 OUT_COLS = dict(x=0, y=1, z=2, d=3, bi=4, yaw=5, yaw_ego=6, aux=7, h=8, w=9, l=10, conf=11,
@@ -120,6 +123,18 @@ SIGNATURES = {
     'ml_iou_matches_host': (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_double, _P, _P, _P, _P]),
     'ml_xyz_from_distance_host': (c_int, [_P, c_int, _P, c_int64, _P]),
     'ml_matching_last_error': (c_char_p, []),
+    'ml_fp8_quantize': (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P]),
+    'ml_fp8_matmul': (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int64, _P, c_int64, c_int, _P, c_int, _P, c_int, c_int64, c_int64,
+                              c_int64, c_int64, _P]),
+    'ml_rms_norm': (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int, c_int64, c_int64, c_float, _P, c_int64, _P, c_int64, _P, c_int64,
+                            _P, c_int64, _P]),
+    'ml_rms_norm_backward_groups': (c_int64, [c_int64, c_int64]),
+    'ml_rms_norm_backward': (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, c_int, c_int64, c_int64, c_float, _P, c_int64, _P,
+                                     _P, _P]),
+    'ml_sum_rows': (c_int, [_P, c_int64, c_int64, _P, c_int, _P]),
+    'ml_adamw_step': (c_int, [c_int, _P, _P, _P, c_int, _P, _P, _P, c_int64, c_double, c_double, c_double, c_double, c_double, c_uint32,
+                              _P]),
+    'ml_ops_last_error': (c_char_p, []),
     'ml_loco_profile_begin': (c_int, [_P, c_int]),
     'ml_loco_profile_end': (c_int, [_P, POINTER(c_int64), POINTER(c_double), POINTER(c_double), POINTER(c_int64), c_int]),
     'ml_debug_linear': (c_int, [_P, c_int64, c_int, POINTER(c_float), POINTER(c_float), c_int, c_int, _P, _P,
@@ -164,6 +179,13 @@ def load():
 def check(code, train=False):
     if code != 0:
         msg = load().ml_train_last_error() if train else load().ml_last_error()
+        raise MonolocoHipError("monoloco_hip error %d: %s" % (code, msg.decode() if msg else '?'))
+
+
+def check_ops(code):
+    """check() for the 8-bit residual-block operators (their error text is ml_ops_last_error's)."""
+    if code != 0:
+        msg = load().ml_ops_last_error()
         raise MonolocoHipError("monoloco_hip error %d: %s" % (code, msg.decode() if msg else '?'))
 
 

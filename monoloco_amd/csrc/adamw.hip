@@ -1,0 +1,217 @@
+// adamw.hip -- one AdamW step over many tensors at once, moments in 32 bits or in e4m3 blocks of 128 (block8.h).
+//
+//   m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) g^2;  p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// (the reference's optimizer is torch.optim.Adam, monoloco/train/trainer.py:128; AdamW decays the weights apart from the gradient.)
+// Bound by memory: per element 3 parameter / gradient accesses and 4 of the moments (28 bytes with fp32 parameters and moments, 10
+// with bf16 parameters and 8-bit moments).  One launch takes up to 64 tensors: their pointers ride in the kernel's arguments (no table
+// to upload, nothing kept between calls), and a workgroup finds its tensor with one load per lane and a ballot.
+//
+// 8-bit moments: m and r = sqrt(v) as codes (r, not v: its range is half as many powers of two).  With b2 = 0.999 a step changes r by
+// less than a code's half step, so rounding to nearest would never move it: both are rounded STOCHASTICALLY, up with the probability
+// of the distance, from 16 + 16 random bits per element that depend on the seed, the step, the tensor's place in the call and the
+// element alone (rng.h's generator).  The update itself uses the unrounded m' and r'.  r' > 0 keeps at least the smallest code: a
+// second moment that vanished would let the next step divide by eps.
+#include "block8.h"
+#include "rng.h"
+
+using namespace mlk;
+
+namespace {
+
+constexpr int MAX_TENSORS = 64;   // lanes of a wave; the table has to fit into the 4 KiB of kernel arguments
+
+struct AdamTable {
+    void* p[MAX_TENSORS];
+    const void* g[MAX_TENSORS];
+    void* m[MAX_TENSORS];
+    void* v[MAX_TENSORS];
+    uint8_t* s[MAX_TENSORS];        // 8-bit moments: scales of m, then of r (blocks each)
+    long numel[MAX_TENSORS];
+    unsigned first[MAX_TENSORS];    // first workgroup of the tensor; behind the last tensor: the grid
+    unsigned key[MAX_TENSORS];      // random key of the tensor; 
+};
+static_assert(sizeof(AdamTable) <= 3700, "kernel arguments");
+
+struct AdamScalars {
+    float b1, c1, b2, c2, size, root, eps, keep;   // c = 1 - b; size = lr / (1 - b1^t); root = sqrt(1 - b2^t); keep = 1 - lr wd
+};
+
+constexpr int WG_ELEMS = 4096;   // elements per workgroup: 256 threads, 2 chunks of 8 each
+
+__device__ __forceinline__ float adam_update(float p, float m, float r, const AdamScalars& a) {
+    return p * a.keep - a.size * m / (r / a.root + a.eps);
+}
+
+// the tensor of this workgroup: the number of tensors that start at or before it, minus one
+__device__ __forceinline__ int tensor_of(const AdamTable& t, unsigned block) {
+    const unsigned f = t.first[threadIdx.x & 63];
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(f <= block)) - 1);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void adamw32_kernel(AdamTable t, AdamScalars a) {
+    const int k = tensor_of(t, blockIdx.x);
+    const long n = t.numel[k], base = (long)(blockIdx.x - t.first[k]) * WG_ELEMS;
+    T* const P = (T*)t.p[k];
+    const T* const G = (const T*)t.g[k];
+    float* const M = (float*)t.m[k];
+    float* const V = (float*)t.v[k];
+    const bool vec = (((uintptr_t)P | (uintptr_t)G | (uintptr_t)M | (uintptr_t)V) & 15) == 0;
+#pragma unroll
+    for (int j = 0; j < WG_ELEMS / 2048; ++j) {
+        const long i = base + j * 2048 + threadIdx.x * 8;
+        if (i >= n) break;
+        float p[8], g[8], m[8], v[8];
+        load8(P + i, n - i, vec, p);
+        load8(G + i, n - i, vec, g);
+        load8(M + i, n - i, vec, m);
+        load8(V + i, n - i, vec, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            m[e] = m[e] * a.b1 + g[e] * a.c1;
+            v[e] = v[e] * a.b2 + g[e] * g[e] * a.c2;
+            p[e] = adam_update(p[e], m[e], sqrtf(v[e]), a);
+        }
+        store8(P + i, n - i, vec, p);
+        store8(M + i, n - i, vec, m);
+        store8(V + i, n - i, vec, v);
+    }
+}
+
+// |x| <= 448 times the scale's inverse -> code, rounded up if the fraction plus u / 2^16 reaches 1
+__device__ __forceinline__ unsigned code_stochastic(float x, unsigned u16) {
+    const unsigned sign = __float_as_uint(x) >> 31 << 7, bits = absbits(x);
+    if (bits >= (121u << 23)) return sign | (((bits + (u16 << 4)) >> 20) - (120u << 3));   // 2^-6 and more: 20 bits behind the mantissa's 3
+    return sign | (((unsigned)(__uint_as_float(bits) * 536870912.0f) + (u16 << 4)) >> 20);   // multiples of 2^-9, 20 bits behind
+}
+__device__ __forceinline__ void decode8(u32x2 c, float scale, float (&x)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], true);
+        x[h * 4] = lo[0] * scale, x[h * 4 + 1] = lo[1] * scale, x[h * 4 + 2] = hi[0] * scale, x[h * 4 + 3] = hi[1] * scale;
+    }
+}
+__device__ __forceinline__ u32x2 load_codes8(const uint8_t* p, long left, bool vec) {
+    if (vec && left >= 8) return *(const u32x2*)p;
+    u32x2 c = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < left) c[i >> 2] |= (unsigned)p[i] << (8 * (i & 3));
+    return c;
+}
+// 8 new values of a moment -> codes and the block's scale (16 lanes = 128 values)
+__device__ __forceinline__ u32x2 encode8(const float (&x)[8], const unsigned (&u)[8], int shift, bool positive, unsigned& byte) {
+    unsigned a = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a = max(a, absbits(x[e]));
+    byte = scale_byte(max16(a));
+    u32x2 c = {0x7f7f7f7fu, 0x7f7f7f7fu};
+    if (byte != 255) {
+        const float inv = scale_inverse(byte);
+        c[0] = c[1] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            unsigned q = code_stochastic(x[e] * inv, u[e] >> shift & 0xffffu);
+            if (positive && q == 0 && x[e] > 0.0f) q = 1;
+            c[e >> 2] |= q << (8 * (e & 3));
+        }
+    }
+    return c;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void adamw8_kernel(AdamTable t, AdamScalars a) {
+    const int k = tensor_of(t, blockIdx.x);
+    const long n = t.numel[k], base = (long)(blockIdx.x - t.first[k]) * WG_ELEMS, blocks = (n + QB - 1) / QB;
+    T* const P = (T*)t.p[k];
+    const T* const G = (const T*)t.g[k];
+    uint8_t* const M = (uint8_t*)t.m[k];
+    uint8_t* const R = (uint8_t*)t.v[k];
+    uint8_t* const SM = t.s[k];
+    uint8_t* const SR = SM + blocks;
+    const unsigned key = t.key[k];
+    const bool vec = (((uintptr_t)P | (uintptr_t)G) & 15) == 0 && (((uintptr_t)M | (uintptr_t)R) & 7) == 0;
+#pragma unroll
+    for (int j = 0; j < WG_ELEMS / 2048; ++j) {
+        const long i = base + j * 2048 + threadIdx.x * 8, b = i / QB;
+        if (b >= blocks) break;   // (16 lanes together)
+        float p[8], g[8], m[8], r[8];
+        load8(P + i, n - i, vec, p);
+        load8(G + i, n - i, vec, g);
+        decode8(load_codes8(M + i, n - i, vec), scale_value(SM[b]), m);
+        decode8(load_codes8(R + i, n - i, vec), scale_value(SR[b]), r);
+        const unsigned bk = mix32(key + (unsigned)b * 0x9e3779b9u);
+        unsigned u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            u[e] = mix32(bk + (unsigned)((i + e) & 127) * 0x85ebca6bu);
+            m[e] = m[e] * a.b1 + g[e] * a.c1;
+            r[e] = sqrtf(r[e] * r[e] * a.b2 + g[e] * g[e] * a.c2);
+            p[e] = adam_update(p[e], m[e], r[e], a);
+        }
+        unsigned bm, br;
+        const u32x2 cm = encode8(m, u, 0, false, bm), cr = encode8(r, u, 16, true, br);
+        if (i < n) {
+            store8(P + i, n - i, vec, p);
+            store_codes8(M + i, n - i, vec, cm);
+            store_codes8(R + i, n - i, vec, cr);
+        }
+        if ((threadIdx.x & 15) == 0) SM[b] = (uint8_t)bm, SR[b] = (uint8_t)br;
+    }
+}
+
+uint32_t host_mix32(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x7feb352dU;
+    x ^= x >> 15;
+    x *= 0x846ca68bU;
+    return x ^ (x >> 16);
+}
+
+}  // namespace
+
+extern "C" int ml_adamw_step(int n_tensors, const int64_t* numel, void* const* params, const void* const* grads, int dtype, void* const* exp_avgs,
+                             void* const* exp_avg_sqs, uint8_t* const* scales, int64_t step, double lr, double beta1, double beta2, double eps,
+                             double weight_decay, uint32_t seed, void* stream) {
+    if (n_tensors < 0 || (dtype != ML_F32 && dtype != ML_BF16 && dtype != ML_F16)) return ops_fail(ML_ERR_ARG, "ml_adamw_step: bad type %d or count %d", dtype, n_tensors);
+    if (n_tensors == 0) return ML_OK;
+    if (!numel || !params || !grads || !exp_avgs || !exp_avg_sqs) return ops_fail(ML_ERR_ARG, "ml_adamw_step: null pointer");
+    if (step < 1) return ops_fail(ML_ERR_ARG, "ml_adamw_step: steps are counted from 1, got %lld", (long long)step);
+    if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0)) return ops_fail(ML_ERR_ARG, "ml_adamw_step: betas are in [0, 1), eps is not negative");
+    for (int i = 0; i < n_tensors; ++i) {
+        if (numel[i] < 0 || numel[i] > (1LL << 38)) return ops_fail(ML_ERR_SHAPE, "ml_adamw_step: tensor %d has %lld elements", i, (long long)numel[i]);
+        if (numel[i] && (!params[i] || !grads[i] || !exp_avgs[i] || !exp_avg_sqs[i] || (scales && !scales[i]))) return ops_fail(ML_ERR_ARG, "ml_adamw_step: tensor %d has a null pointer", i);
+    }
+    const hipStream_t s = (hipStream_t)stream;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    const hipError_t ce = hipStreamIsCapturing(s, &cap);
+    if (ce != hipSuccess) return ops_fail(ML_ERR_HIP, "ml_adamw_step: %s", hipGetErrorString(ce));
+    if (cap != hipStreamCaptureStatusNone) return ops_fail(ML_ERR_STATE, "ml_adamw_step: the step's number is part of the launch; a captured one would repeat it");
+    const AdamScalars a{(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), (float)(lr / (1 - pow(beta1, (double)step))),
+                        (float)sqrt(1 - pow(beta2, (double)step)), (float)eps, (float)(1 - lr * weight_decay)};
+    for (int i = 0; i < n_tensors;) {
+        AdamTable t;
+        unsigned grid = 0;
+        int k = 0;
+        for (; i < n_tensors && k < MAX_TENSORS; ++i) {
+            if (numel[i] == 0) continue;
+            const int64_t wgs = (numel[i] + WG_ELEMS - 1) / WG_ELEMS;
+            if (k > 0 && grid + wgs > 0x7fffffffLL) break;   // (one tensor alone always fits: at most 2^26 workgroups)
+            t.p[k] = params[i], t.g[k] = grads[i], t.m[k] = exp_avgs[i], t.v[k] = exp_avg_sqs[i], t.s[k] = scales ? scales[i] : nullptr;
+            t.numel[k] = numel[i], t.first[k] = grid;
+            t.key[k] = host_mix32(seed + 0x9e3779b9U * host_mix32((uint32_t)step + 0x85ebca6bU * (uint32_t)(i + 1)));
+            grid += (unsigned)wgs;
+            ++k;
+        }
+        if (k == 0) break;
+        for (; k < MAX_TENSORS; ++k) t.first[k] = 0xffffffffu;
+        const bool eight = scales != nullptr;
+        if (dtype == ML_F32) { if (eight) adamw8_kernel<float><<<grid, 256, 0, s>>>(t, a); else adamw32_kernel<float><<<grid, 256, 0, s>>>(t, a); }
+        else if (dtype == ML_BF16) { if (eight) adamw8_kernel<bf16_t><<<grid, 256, 0, s>>>(t, a); else adamw32_kernel<bf16_t><<<grid, 256, 0, s>>>(t, a); }
+        else { if (eight) adamw8_kernel<f16_t><<<grid, 256, 0, s>>>(t, a); else adamw32_kernel<f16_t><<<grid, 256, 0, s>>>(t, a); }
+        const int rc = ops_launched("ml_adamw_step");
+        if (rc) return rc;
+    }
+    return ML_OK;
+}

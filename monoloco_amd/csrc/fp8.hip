@@ -1,0 +1,171 @@
+// fp8.hip -- C entry points of the 8-bit residual-block operators: quantisation into e4m3 blocks of 128, the block-scaled product,
+// root-mean-square norm with residual (8-bit or plain output) and its backward pass.  All are asynchronous on the caller's stream,
+// allocate nothing and keep nothing between calls (a workspace is an argument), so they may be captured into a graph.
+#include "fp8_gemm.h"
+#include "fp8_quant.h"
+#include "norm_kernels.h"
+
+using namespace mlk;
+
+namespace {
+
+constexpr long MAX_GRID = 0x7fffffffL;
+
+int elem_size(int dtype) { return dtype == ML_F32 ? 4 : dtype == ML_BF16 || dtype == ML_F16 ? 2 : 0; }
+
+bool rows_aligned(const void* p, long ld, int es, int to) { return !p || (((uintptr_t)p % to) == 0 && (ld * es) % to == 0); }
+
+// f(T{}) for the element type
+template <typename F>
+void with_type(int dtype, F f) {
+    if (dtype == ML_F32) f(float{});
+    else if (dtype == ML_BF16) f(bf16_t{});
+    else f(f16_t{});
+}
+
+template <typename T, bool OUT8>
+void launch_norm(const NormParams& p, hipStream_t s) {
+    const unsigned g4 = (unsigned)((p.m + 3) / 4), g1 = (unsigned)p.m;
+    if (p.n <= 512) rms_norm_kernel<T, OUT8, 1, 1><<<g4, 256, 0, s>>>(p);
+    else if (p.n <= 1024) rms_norm_kernel<T, OUT8, 1, 2><<<g4, 256, 0, s>>>(p);
+    else if (p.n <= 2048) rms_norm_kernel<T, OUT8, 1, 4><<<g4, 256, 0, s>>>(p);
+    else if (p.n <= 4096) rms_norm_kernel<T, OUT8, 4, 2><<<g1, 256, 0, s>>>(p);
+    else if (p.n <= 8192) rms_norm_kernel<T, OUT8, 4, 4><<<g1, 256, 0, s>>>(p);
+    else if (p.n <= 32768) rms_norm_kernel<T, OUT8, 16, 4><<<g1, 1024, 0, s>>>(p);
+    else rms_norm_kernel<T, OUT8, 16, 0><<<g1, 1024, 0, s>>>(p);
+}
+
+template <typename T>
+void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
+    if (p.n <= 512) rms_norm_back_kernel<T, 1, 1><<<g, 256, 0, s>>>(p);
+    else if (p.n <= 1024) rms_norm_back_kernel<T, 1, 2><<<g, 256, 0, s>>>(p);
+    else if (p.n <= 2048) rms_norm_back_kernel<T, 1, 4><<<g, 256, 0, s>>>(p);
+    else if (p.n <= 4096) rms_norm_back_kernel<T, 4, 2><<<g, 256, 0, s>>>(p);
+    else if (p.n <= 8192) rms_norm_back_kernel<T, 4, 4><<<g, 256, 0, s>>>(p);
+    else if (p.n <= 32768) rms_norm_back_kernel<T, 16, 4><<<g, 1024, 0, s>>>(p);
+    else rms_norm_back_kernel<T, 16, 0><<<g, 1024, 0, s>>>(p);
+}
+
+// workgroups of the backward pass = rows of its partial sums: enough to fill 256 CUs with 16 waves, few enough that writing and
+// joining their sums stays below a thirtieth of the traffic from 32768 rows on
+long norm_groups(long m, long n) {
+    const long teams = n <= 2048 ? 4 : 1, most = n <= 8192 ? 1024 : 512;
+    const long g = (m + teams - 1) / teams;
+    return g < most ? g : most;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* ml_ops_last_error(void) { return g_ops_err; }
+
+int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t ldx, int tile, uint8_t* q_dev, int64_t ldq,
+                    uint8_t* scale_dev, int64_t lds, uint8_t* qt_dev, int64_t ldqt, uint8_t* scale_t_dev, int64_t ldst,
+                    float* colsum_dev, void* stream) {
+    const int es = elem_size(dtype);
+    if (!es || m < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_fp8_quantize: bad type %d or size %lld x %lld", dtype, (long long)m, (long long)n);
+    if (m == 0 || n == 0) return ML_OK;
+    if (!x_dev || (!q_dev && !qt_dev) || (q_dev && !scale_dev) || (qt_dev && !scale_t_dev)) return ops_fail(ML_ERR_ARG, "ml_fp8_quantize: null pointer");
+    const long nb = (n + QB - 1) / QB, mb = (m + QB - 1) / QB;
+    if (ldx < n || (q_dev && (ldq < n || lds < nb)) || (qt_dev && (ldqt < m || ldst < mb)))
+        return ops_fail(ML_ERR_ARG, "ml_fp8_quantize: a row stride is shorter than its row");
+    if (m > (1LL << 40) || n > (1LL << 40)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_quantize: %lld x %lld is too large", (long long)m, (long long)n);
+    QuantParams p{};
+    p.x = x_dev, p.m = m, p.n = n, p.ldx = ldx, p.tile = tile != 0;
+    p.q = q_dev, p.scale = scale_dev, p.ldq = ldq, p.lds = lds;
+    p.qt = qt_dev, p.scale_t = scale_t_dev, p.ldqt = ldqt, p.ldst = ldst, p.colsum = colsum_dev;
+    p.vec = rows_aligned(x_dev, ldx, es, 16), p.vecq = rows_aligned(q_dev, ldq, 1, 8), p.vecqt = rows_aligned(qt_dev, ldqt, 1, 8);
+    const hipStream_t s = (hipStream_t)stream;
+    const bool rows = !qt_dev && !tile && !colsum_dev;
+    const long grid = rows ? (m * nb + 15) / 16 : mb * nb;
+    if (grid > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_fp8_quantize: %lld x %lld is too large", (long long)m, (long long)n);
+    with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (rows) quantize_rows_kernel<T><<<(unsigned)grid, 256, 0, s>>>(p);
+        else quantize_tile_kernel<T><<<(unsigned)grid, 256, 0, s>>>(p);
+    });
+    return ops_launched("ml_fp8_quantize");
+}
+
+int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
+                  const uint8_t* b_scale_dev, int64_t ldsb, int b_tile, const void* bias_dev, int bias_dtype, void* c_dev, int c_dtype,
+                  int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream) {
+    const int es = elem_size(c_dtype);
+    if (!es || (bias_dev && !elem_size(bias_dtype)) || m < 0 || n < 0 || k < 0) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: bad type %d, %d or size", c_dtype, bias_dtype);
+    if (m == 0 || n == 0) return ML_OK;
+    if (!c_dev || (k > 0 && (!a_dev || !b_dev || !a_scale_dev || !b_scale_dev))) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: null pointer");
+    const long kb = (k + QB - 1) / QB;
+    if (lda < k || ldb < k || ldc < n || ldsa < kb || ldsb < kb) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: a row stride is shorter than its row");
+    const long grid = ((m + 63) / 64) * ((n + 63) / 64);
+    if (m > (1LL << 40) || n > (1LL << 40) || grid > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
+    GemmParams p{a_dev, b_dev, a_scale_dev, b_scale_dev, (long)lda, (long)ldb, (long)ldsa, (long)ldsb, a_tile != 0, b_tile != 0, bias_dev, bias_dtype, c_dev,
+                 (long)m, (long)n, (long)k, (long)ldc, 0, 0, 0};
+    p.fast_a = rows_aligned(a_dev, lda, 1, 16), p.fast_b = rows_aligned(b_dev, ldb, 1, 16), p.vec_c = rows_aligned(c_dev, ldc, es, 16);
+    const hipStream_t s = (hipStream_t)stream;
+    with_type(c_dtype, [&](auto t) { fp8_gemm64_kernel<decltype(t)><<<(unsigned)grid, 256, 0, s>>>(p); });
+    return ops_launched("ml_fp8_matmul");
+}
+
+int ml_rms_norm(const void* x_dev, int64_t ldx, const void* residual_dev, int64_t ldr, int dtype, const void* w_dev, int w_dtype, int64_t m,
+                int64_t n, float eps, void* h_dev, int64_t ldh, void* y_dev, int64_t ldy, uint8_t* q_dev, int64_t ldq, uint8_t* scale_dev,
+                int64_t lds, void* stream) {
+    const int es = elem_size(dtype);
+    if (!es || (w_dtype != dtype && w_dtype != ML_F32) || m < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_rms_norm: bad types %d, %d or size", dtype, w_dtype);
+    if (m == 0 || n == 0) return ML_OK;
+    if (!x_dev || !w_dev || (!y_dev == !q_dev) || (q_dev && !scale_dev)) return ops_fail(ML_ERR_ARG, "ml_rms_norm: null pointer, or not one of y and q");
+    const long nb = (n + QB - 1) / QB;
+    if (ldx < n || (residual_dev && ldr < n) || (h_dev && ldh < n) || (y_dev && ldy < n) || (q_dev && (ldq < n || lds < nb)))
+        return ops_fail(ML_ERR_ARG, "ml_rms_norm: a row stride is shorter than its row");
+    if (m > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm: %lld rows are too many", (long long)m);
+    NormParams p{};
+    p.x = x_dev, p.residual = residual_dev, p.w = w_dev, p.w_f32 = w_dtype == ML_F32;
+    p.m = m, p.n = n, p.ldx = ldx, p.ldr = ldr, p.ldy = q_dev ? ldq : ldy, p.ldh = ldh, p.eps = eps;
+    p.y = y_dev, p.h = h_dev, p.q = q_dev, p.scale = scale_dev, p.lds = lds;
+    p.vec = rows_aligned(x_dev, ldx, es, 16) && rows_aligned(residual_dev, ldr, es, 16) && rows_aligned(h_dev, ldh, es, 16) &&
+            rows_aligned(y_dev, ldy, es, 16) && rows_aligned(q_dev, ldq, 1, 8) && ((uintptr_t)w_dev % 16) == 0;
+    const hipStream_t s = (hipStream_t)stream;
+    with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (q_dev) launch_norm<T, true>(p, s);
+        else launch_norm<T, false>(p, s);
+    });
+    return ops_launched("ml_rms_norm");
+}
+
+int64_t ml_rms_norm_backward_groups(int64_t m, int64_t n) { return m <= 0 || n <= 0 ? 0 : norm_groups(m, n); }
+
+int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int64_t ldh, const void* dh_dev, int64_t ldd, int dtype,
+                         const void* w_dev, int w_dtype, int64_t m, int64_t n, float eps, void* dx_dev, int64_t ldx, void* dw_dev,
+                         float* work_dev, void* stream) {
+    const int es = elem_size(dtype);
+    if (!es || (w_dtype != dtype && w_dtype != ML_F32) || m < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: bad types %d, %d or size", dtype, w_dtype);
+    if (n == 0) return ML_OK;
+    if (!dw_dev || (m > 0 && (!dy_dev || !h_dev || !w_dev || !dx_dev || !work_dev))) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: null pointer");
+    if (m > 0 && (ldy < n || ldh < n || (dh_dev && ldd < n) || ldx < n)) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: a row stride is shorter than its row");
+    const hipStream_t s = (hipStream_t)stream;
+    const long groups = m ? norm_groups(m, n) : 0;
+    if (m > 0) {
+        NormBackParams p{};
+        p.dy = dy_dev, p.h = h_dev, p.w = w_dev, p.dh = dh_dev, p.w_f32 = w_dtype == ML_F32;
+        p.m = m, p.n = n, p.ldy = ldy, p.ldh = ldh, p.ldd = ldd, p.ldx = ldx, p.eps = eps, p.dx = dx_dev, p.part = work_dev;
+        p.vec = rows_aligned(dy_dev, ldy, es, 16) && rows_aligned(h_dev, ldh, es, 16) && rows_aligned(dh_dev, ldd, es, 16) &&
+                rows_aligned(dx_dev, ldx, es, 16) && ((uintptr_t)w_dev % 16) == 0;
+        with_type(dtype, [&](auto t) { launch_norm_back<decltype(t)>(p, (unsigned)groups, s); });
+        const int rc = ops_launched("ml_rms_norm_backward");
+        if (rc) return rc;
+    }
+    with_type(w_dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + 31) / 32), 1024, 0, s>>>(work_dev, groups, n, (decltype(t)*)dw_dev); });
+    return ops_launched("ml_rms_norm_backward");
+}
+
+int ml_sum_rows(const float* part_dev, int64_t rows, int64_t n, void* out_dev, int dtype, void* stream) {
+    if (!elem_size(dtype) || rows < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_sum_rows: bad type %d or size", dtype);
+    if (n == 0) return ML_OK;
+    if (!out_dev || (rows > 0 && !part_dev)) return ops_fail(ML_ERR_ARG, "ml_sum_rows: null pointer");
+    if ((n + 31) / 32 > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_sum_rows: %lld columns are too many", (long long)n);
+    with_type(dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + 31) / 32), 1024, 0, (hipStream_t)stream>>>(part_dev, rows, n, (decltype(t)*)out_dev); });
+    return ops_launched("ml_sum_rows");
+}
+
+}  // extern "C"

@@ -1,0 +1,125 @@
+// fp8_quant.h -- fp32 / bf16 / fp16 matrices -> e4m3 blocks of 128 (block8.h): along rows (1 x 128), as 128 x 128 tiles, and the
+// transposed matrix in the same pass (a backward product reduces over the other axis, and the matrix instruction wants both
+// operands contiguous along the reduction).  Bound by memory: every element is read once, also where two forms are written.
+#pragma once
+#include "block8.h"
+
+namespace mlk {
+
+struct QuantParams {
+    const void* x;      // (m, n), row stride ldx
+    long m, n, ldx;
+    int tile;           // one scale per 128 x 128 instead of 1 x 128
+    uint8_t* q;         // (m, n), row stride ldq, or null
+    uint8_t* scale;     // (m, nb) or (mb, nb), row stride lds
+    long ldq, lds;
+    uint8_t* qt;        // (n, m), row stride ldqt, or null
+    uint8_t* scale_t;   // (n, mb) or (nb, mb), row stride ldst
+    long ldqt, ldst;
+    float* colsum;      // (mb, n): column sums of every 128 rows, or null
+    int vec, vecq, vecqt;
+};
+
+// rows only: 16 lanes per block of 128, no LDS
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantParams p) {
+    const long nb = (p.n + QB - 1) / QB, units = p.m * nb;
+    const long u = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (u >= units) return;   // (whole groups of 16 lanes)
+    const long row = u / nb, b = u - row * nb, c = b * QB + (threadIdx.x & 15) * 8;
+    float x[8];
+    load8((const T*)p.x + row * p.ldx + c, p.n - c, p.vec, x);
+    unsigned a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max(a, absbits(x[i]));
+    const unsigned byte = scale_byte(max16(a));
+    if (c < p.n) store_codes8(p.q + row * p.ldq + c, p.n - c, p.vecq, codes8(x, byte));
+    if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + b] = (uint8_t)byte;
+}
+
+// a 128 x 128 tile per workgroup of 256 threads: thread (tr, tc) = (t / 16, t % 16) holds rows 8 tr .. + 7, columns 8 tc .. + 7
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_tile_kernel(QuantParams p) {
+    constexpr int PITCH = QB + 8;
+    __shared__ unsigned cmax[4][QB];
+    __shared__ float csum[4][QB];
+    __shared__ __attribute__((aligned(16))) uint8_t tq[QB * PITCH];
+    const int tc = threadIdx.x & 15, tr = threadIdx.x >> 4, wave = threadIdx.x >> 6;
+    const long nb = (p.n + QB - 1) / QB, mb = (p.m + QB - 1) / QB;
+    const long bi = blockIdx.x / nb, bj = blockIdx.x - bi * nb;
+    const long r0 = bi * QB + tr * 8, c0 = bj * QB + tc * 8;
+    float x[8][8];
+    unsigned rmax[8], colmax[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        load8((const T*)p.x + (r0 + i) * p.ldx + c0, r0 + i < p.m ? p.n - c0 : 0, p.vec, x[i]);
+        rmax[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            rmax[i] = max(rmax[i], absbits(x[i][j]));
+            colmax[j] = max(colmax[j], absbits(x[i][j]));
+        }
+        rmax[i] = max16(rmax[i]);
+    }
+    // columns (and sums): over the four row groups of a wave, then over the four waves
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        colmax[j] = max(colmax[j], (unsigned)__shfl_xor((int)colmax[j], 16));
+        colmax[j] = max(colmax[j], (unsigned)__shfl_xor((int)colmax[j], 32));
+        if ((threadIdx.x & 48) == 0) cmax[wave][tc * 8 + j] = colmax[j];
+        if (p.colsum) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += x[i][j];
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if ((threadIdx.x & 48) == 0) csum[wave][tc * 8 + j] = s;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int c = tc * 8 + j;
+        colmax[j] = max(max(cmax[0][c], cmax[1][c]), max(cmax[2][c], cmax[3][c]));
+        if (p.colsum && tr == 0 && c0 + j < p.n) p.colsum[bi * p.n + c0 + j] = (csum[0][c] + csum[1][c]) + (csum[2][c] + csum[3][c]);
+    }
+    unsigned tb = 0;
+    if (p.tile) {
+        unsigned a = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a = max(a, colmax[j]);
+        tb = scale_byte(max16(a));
+    }
+    if (p.q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned byte = p.tile ? tb : scale_byte(rmax[i]);
+            if (r0 + i < p.m && c0 < p.n) store_codes8(p.q + (r0 + i) * p.ldq + c0, p.n - c0, p.vecq, codes8(x[i], byte));
+            if (!p.tile && tc == 0 && r0 + i < p.m) p.scale[(r0 + i) * p.lds + bj] = (uint8_t)byte;
+        }
+        if (p.tile && threadIdx.x == 0) p.scale[bi * p.lds + bj] = (uint8_t)tb;
+    }
+    if (p.qt) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const unsigned byte = p.tile ? tb : scale_byte(colmax[j]);
+            float col[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) col[i] = x[i][j];
+            *(u32x2*)(tq + (tc * 8 + j) * PITCH + tr * 8) = codes8(col, byte);
+            if (!p.tile && tr == 0 && c0 + j < p.n) p.scale_t[(c0 + j) * p.ldst + bi] = (uint8_t)byte;
+        }
+        if (p.tile && threadIdx.x == 0) p.scale_t[bj * p.ldst + bi] = (uint8_t)tb;
+        __syncthreads();
+        // row c of the transposed tile: 16 lanes x 8 bytes
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int c = tr + 16 * k;
+            const long rt = bj * QB + c, ct = bi * QB + tc * 8;
+            if (rt < p.n && ct < p.m) store_codes8(p.qt + rt * p.ldqt + ct, p.m - ct, p.vecqt, *(const u32x2*)(tq + c * PITCH + tc * 8));
+        }
+    }
+    (void)mb;
+}
+
+}  // namespace mlk

@@ -1,0 +1,262 @@
+// norm_kernels.h -- root-mean-square norm over the last axis, with the residual's addition, forward and backward.
+//
+//   h = x + residual;  rstd = 1 / sqrt(mean_j h_j^2 + eps);  y_j = h_j rstd w_j          (y, statistics from h before its rounding)
+//   g = dy * w;  dx_j = rstd (g_j - h_j rstd^2 mean_i(g_i h_i)) + dh_j;   dw_j = sum over rows of dy_j h_j rstd
+//
+// Bound by memory: forward 2 reads + 2 writes per element (8-bit output: one byte instead of the last), backward 3 reads + 1 write.
+// A row stays in registers between its reduction and its output, so everything is read once.  A lane owns chunks of 8 consecutive
+// elements (one 16-byte access of a 2-byte type; 16 neighbouring lanes = one block of 128 of the 8-bit output, whose maximum is
+// four DPP rotations).  WPR = waves per row, NV = chunks per lane: a row of up to 2048 elements is one wave's (no LDS, no barrier;
+// four rows per workgroup), longer ones take 4 or 16 waves; NV = 0 streams rows beyond 32768 elements from memory twice.
+#pragma once
+#include "block8.h"
+
+namespace mlk {
+
+struct NormParams {
+    const void* x;          // (m, n), row stride ldx
+    const void* residual;   // or null
+    const void* w;          // (n)
+    int w_f32;              // w is fp32 (else x's type)
+    long m, n, ldx, ldr, ldy, ldh;
+    float eps;
+    void* y;                // (m, n) in x's type, or null
+    void* h;                // (m, n) in x's type, or null
+    uint8_t* q;             // (m, n) codes, or null
+    uint8_t* scale;         // (m, blocks), row stride lds
+    long lds;
+    int vec;                // every operand's rows are 16-byte aligned (q: 8)
+};
+
+template <int WPR>
+__device__ __forceinline__ float row_sum(float x, float* red) {
+    x = wave_sum(x);
+    if (WPR == 1) return x;
+    __syncthreads();   // (the previous reduction's readers are done)
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WPR; ++i) s += red[i];
+    return s;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_weight8(const void* w, int w_f32, long c, long n, bool vec, float (&x)[8]) {
+    if (w_f32) load8((const float*)w + c, n - c, vec, x);
+    else load8((const T*)w + c, n - c, vec, x);
+}
+
+// one chunk's output
+template <typename T, bool OUT8>
+__device__ __forceinline__ void norm_out(const NormParams& p, long row, long c, const float (&h)[8], float rstd) {
+    float wv[8], y[8];
+    load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = h[i] * rstd * wv[i];
+    if (OUT8) {
+        unsigned a = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = max(a, c + i < p.n ? absbits(y[i]) : 0u);
+        const unsigned byte = scale_byte(max16(a));
+        if (c < p.n) {
+            store_codes8(p.q + row * p.ldy + c, p.n - c, p.vec, codes8(y, byte));
+            if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + c / QB] = (uint8_t)byte;
+        }
+    } else if (c < p.n) {
+        store8((T*)p.y + row * p.ldy + c, p.n - c, p.vec, y);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void norm_in(const NormParams& p, long row, long c, float (&h)[8]) {
+    load8((const T*)p.x + row * p.ldx + c, p.n - c, p.vec, h);
+    if (p.residual) {
+        float r[8];
+        load8((const T*)p.residual + row * p.ldr + c, p.n - c, p.vec, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] += r[i];
+    }
+}
+
+template <typename T, bool OUT8, int WPR, int NV>
+__global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_kernel(NormParams p) {
+    __shared__ float red[WPR];
+    const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;   // place in the row's team
+    const long row = WPR == 1 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= p.m) return;   // (WPR > 1: never taken, the grid is m)
+    constexpr long STEP = WPR * 64 * 8;
+    float ss = 0.0f;
+    if constexpr (NV > 0) {
+        float h[NV][8];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            norm_in<T>(p, row, lane * 8 + j * STEP, h[j]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += h[j][i] * h[j][i];
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<WPR>(ss, red) / (float)p.n + p.eps);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const long c = lane * 8 + j * STEP;
+            if (p.h && c < p.n) store8((T*)p.h + row * p.ldh + c, p.n - c, p.vec, h[j]);
+            norm_out<T, OUT8>(p, row, c, h[j], rstd);
+        }
+    } else {   // long rows: once for the sum, once for the output
+        const long end = (p.n + STEP - 1) / STEP * STEP;   // (whole teams: the block maximum needs its 16 lanes)
+        float h[8];
+        for (long c = lane * 8; c < end; c += STEP) {
+            norm_in<T>(p, row, c, h);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += h[i] * h[i];
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<WPR>(ss, red) / (float)p.n + p.eps);
+        for (long c = lane * 8; c < end; c += STEP) {
+            norm_in<T>(p, row, c, h);
+            if (p.h && c < p.n) store8((T*)p.h + row * p.ldh + c, p.n - c, p.vec, h);
+            norm_out<T, OUT8>(p, row, c, h, rstd);
+        }
+    }
+}
+
+struct NormBackParams {
+    const void* dy;   // (m, n)
+    const void* h;    // (m, n): what the forward pass wrote (or its input, without a residual)
+    const void* w;
+    const void* dh;   // or null
+    int w_f32;
+    long m, n, ldy, ldh, ldd, ldx;
+    float eps;
+    void* dx;         // (m, n)
+    float* part;      // (groups, n) partial sums of dw
+    int vec;
+};
+
+// A workgroup takes rows g, g + groups, ...; a lane keeps its columns' part of dw in registers over all of them.  The partial sums
+// are joined by reduce_rows_kernel in a fixed order: no atomics, the same bits every time.
+template <typename T, int WPR, int NV>
+__global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kernel(NormBackParams p) {
+    constexpr int TEAMS = WPR == 1 ? 4 : 1;
+    constexpr long STEP = WPR * 64 * 8;
+    __shared__ float red[WPR];
+    __shared__ float sums[TEAMS == 1 ? 1 : 3 * STEP * (NV ? NV : 1)];
+    const int team = WPR == 1 ? threadIdx.x >> 6 : 0;
+    const int lane = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const float inv_n = 1.0f / (float)p.n;
+    float* const part = p.part + (long)blockIdx.x * p.n;
+    if constexpr (NV > 0) {
+        float dw[NV][8] = {};
+        for (long row = (long)blockIdx.x * TEAMS + team; row < p.m; row += (long)gridDim.x * TEAMS) {
+            float h[NV][8], g[NV][8], ss = 0.0f, gh = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const long c = lane * 8 + j * STEP;
+                load8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec, h[j]);
+                load8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec, g[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                float wv[8];
+                load_weight8<T>(p.w, p.w_f32, lane * 8 + j * STEP, p.n, p.vec, wv);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ss += h[j][i] * h[j][i];
+                    gh += g[j][i] * wv[i] * h[j][i];
+                }
+            }
+            ss = row_sum<WPR>(ss, red);
+            gh = row_sum<WPR>(gh, red);
+            const float rstd = 1.0f / sqrtf(ss * inv_n + p.eps);
+            const float k = rstd * rstd * (gh * inv_n);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const long c = lane * 8 + j * STEP;
+                float wv[8], d[8];
+                load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
+                if (p.dh) load8((const T*)p.dh + row * p.ldd + c, p.n - c, p.vec, d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    dw[j][i] += g[j][i] * (h[j][i] * rstd);
+                    const float v = rstd * (g[j][i] * wv[i] - h[j][i] * k);
+                    d[i] = p.dh ? v + d[i] : v;
+                }
+                if (c < p.n) store8((T*)p.dx + row * p.ldx + c, p.n - c, p.vec, d);
+            }
+        }
+        if (TEAMS > 1) {
+            if (team > 0) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sums[(team - 1) * STEP * NV + (j * 8 + i) * 64 + lane] = dw[j][i];
+            }
+            __syncthreads();
+            if (team > 0) return;
+#pragma unroll
+            for (int t = 0; t < TEAMS - 1; ++t)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dw[j][i] += sums[t * STEP * NV + (j * 8 + i) * 64 + lane];
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane * 8 + j * STEP + i < p.n) part[lane * 8 + j * STEP + i] = dw[j][i];
+    } else {
+        bool first = true;   // (the workgroup's own row of `part` carries the sums: no other workgroup touches it)
+        for (long row = blockIdx.x; row < p.m; row += gridDim.x, first = false) {
+            float h[8], g[8], wv[8], ss = 0.0f, gh = 0.0f;
+            for (long c = lane * 8; c < p.n; c += STEP) {
+                load8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec, h);
+                load8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec, g);
+                load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ss += h[i] * h[i];
+                    gh += g[i] * wv[i] * h[i];
+                }
+            }
+            ss = row_sum<WPR>(ss, red);
+            gh = row_sum<WPR>(gh, red);
+            const float rstd = 1.0f / sqrtf(ss * inv_n + p.eps);
+            const float k = rstd * rstd * (gh * inv_n);
+            for (long c = lane * 8; c < p.n; c += STEP) {
+                float d[8];
+                load8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec, h);
+                load8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec, g);
+                load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
+                if (p.dh) load8((const T*)p.dh + row * p.ldd + c, p.n - c, p.vec, d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (c + i < p.n) part[c + i] = (first ? 0.0f : part[c + i]) + g[i] * (h[i] * rstd);
+                    const float v = rstd * (g[i] * wv[i] - h[i] * k);
+                    d[i] = p.dh ? v + d[i] : v;
+                }
+                store8((T*)p.dx + row * p.ldx + c, p.n - c, p.vec, d);
+            }
+        }
+    }
+}
+
+// out[c] = sum over g of part[g * n + c], in a fixed order: 32 columns per workgroup, 32 teams take g = t, t + 32, ...
+template <typename T>
+__global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restrict__ part, long groups, long n, T* __restrict__ out) {
+    __shared__ float s[32][33];
+    const int cx = threadIdx.x & 31, t = threadIdx.x >> 5;
+    const long c = (long)blockIdx.x * 32 + cx;
+    float a = 0.0f;
+    if (c < n)
+        for (long g = t; g < groups; g += 32) a += part[g * n + c];
+    s[t][cx] = a;
+    __syncthreads();
+    if (t == 0 && c < n) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v += s[i][cx];
+        out[c] = (T)v;
+    }
+}
+
+}  // namespace mlk

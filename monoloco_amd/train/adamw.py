@@ -1,0 +1,119 @@
+"""AdamW over many tensors in one launch (``ml_adamw_step``), moments in 32 bits or in the 8-bit blocks of ``monoloco_amd.fp8``.
+
+For the loop a caller owns (``outputs = model(inputs)``; ``loss.backward()``; ``optimizer.step()``): the reference builds torch's Adam
+there (monoloco/train/trainer.py:128-131).  ``HipTrainer`` has its own Adam inside the library and does not need this one."""
+import ctypes
+
+import torch
+
+from .. import _lib
+from .._lib import MonolocoHipError, check_ops
+from ..engine import _stream
+from ..fp8 import BLOCK, CODES, DTYPES, SCALES, _need
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def state_scales(numel, device):
+    """Scales of the 8-bit moments of a tensor of `numel` elements: row 0 for exp_avg, row 1 for the root of exp_avg_sq; all 1."""
+    return torch.ones((2, -(-numel // BLOCK)), device=device).to(SCALES)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, seed=0):
+    """One AdamW step in place: ``step`` counts from 1, all tensors of one type (fp32, bf16, fp16) and device, contiguous, none twice.
+
+    Without ``scales`` the moments are fp32 tensors like the parameters.  With ``scales`` (one (2, ceil(numel / 128)) tensor of e8m0 for
+    each parameter, see ``state_scales``) they are e4m3 codes: exp_avgs of the first moment, exp_avg_sqs of the ROOT of the second, both
+    rounded stochastically from ``seed``, the step, the tensor's place in the lists and the element (the same call gives the same bits).
+    Refused while its stream is captured: the step's number is part of the launch."""
+    k = len(params)
+    _need(len(grads) == k and len(exp_avgs) == k and len(exp_avg_sqs) == k and (scales is None or len(scales) == k),
+          "adamw_step: %d parameters, %d gradients, %d and %d moments", k, len(grads), len(exp_avgs), len(exp_avg_sqs))
+    _need(int(step) >= 1, "adamw_step: steps are counted from 1, got %r", step)
+    if not k:
+        return
+    dev, dt = params[0].device, params[0].dtype
+    if dev.type != 'cuda':
+        raise MonolocoHipError("adamw_step runs on HIP devices only, got a tensor on %s (there is no CPU fallback)" % (dev,))
+    _need(dt in DTYPES, "adamw_step: parameters are fp32, bf16 or fp16, got %s", dt)
+    mdt = torch.float32 if scales is None else CODES
+    sizes = [p.numel() for p in params]
+    for p, g, m, v, n in zip(params, grads, exp_avgs, exp_avg_sqs, sizes):
+        _need(p.dtype == dt and g.dtype == dt and m.dtype == mdt and v.dtype == mdt, "adamw_step: %s parameters take %s gradients and %s moments, got %s, %s, %s, %s",
+              dt, dt, mdt, p.dtype, g.dtype, m.dtype, v.dtype)
+        _need(p.device == dev and g.device == dev and m.device == dev and v.device == dev, "adamw_step: tensors on several devices")
+        _need(p.is_contiguous() and m.is_contiguous() and v.is_contiguous(), "adamw_step: parameters and moments have to be contiguous")
+        _need(g.numel() == n and m.numel() == n and v.numel() == n, "adamw_step: a gradient or moment of another size than its parameter")
+    if scales is not None:
+        for s, n in zip(scales, sizes):
+            _need(s.dtype == SCALES and s.device == dev and s.is_contiguous() and tuple(s.shape) == (2, -(-n // BLOCK)),
+                  "adamw_step: the scales of %d elements are a contiguous (2, %d) of %s on %s, got %s %s", n, -(-n // BLOCK), SCALES, dev, tuple(s.shape), s.dtype)
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    ps, gs, ms, vs = _pointers(params), _pointers(grads), _pointers(exp_avgs), _pointers(exp_avg_sqs)
+    written = [a for t in (ps, ms, vs) for a, n in zip(t, sizes) if n]
+    _need(len(set(written)) == len(written), "adamw_step: a tensor is given twice")
+    with torch.cuda.device(dev):
+        check_ops(_lib.load().ml_adamw_step(
+            k, (ctypes.c_int64 * k)(*sizes), ps, gs, DTYPES[dt], ms, vs, None if scales is None else _pointers(scales),
+            int(step), float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(seed) & 0xffffffff, _stream(dev)))
+    torch.autograd.graph.increment_version(params)   # (LocoModel re-packs its engine when a parameter's version moved)
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW``'s arguments, groups, schedulers and state_dict on ``adamw_step``.
+
+    ``state_bits=8`` keeps the moments as e4m3 blocks (2 + 1/64 bytes per parameter instead of 8); ``seed`` is their rounding's.
+    Parameters that got no gradient are left as they are, each counts its own steps."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
+        _need(state_bits in (8, 32), "AdamW: moments have 8 or 32 bits, not %r", state_bits)
+        _need(lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas), "AdamW: lr, eps and weight_decay are not negative, betas are in [0, 1)")
+        self.state_bits, self.seed = state_bits, int(seed)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _state(self, p):
+        s = self.state[p]
+        if not s:
+            s['step'] = 0
+            dt = torch.float32 if self.state_bits == 32 else CODES
+            for key in ('exp_avg', 'exp_avg_sq'):
+                s[key] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(dt)
+            if self.state_bits == 8:
+                s['scales'] = state_scales(p.numel(), p.device)
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            calls = {}
+            for p in group['params']:
+                if p.grad is None:
+                    continue
+                _need(not p.grad.is_sparse, "AdamW: sparse gradients are not supported")
+                s = self._state(p)
+                calls.setdefault((p.device, p.dtype, s['step'] + 1), []).append((p, s))
+            for (_, _, step), found in calls.items():
+                adamw_step([p for p, _ in found], [p.grad for p, _ in found], [s['exp_avg'] for _, s in found], [s['exp_avg_sq'] for _, s in found],
+                           [s['scales'] for _, s in found] if self.state_bits == 8 else None, step=step, lr=float(group['lr']), betas=group['betas'],
+                           eps=group['eps'], weight_decay=group['weight_decay'], seed=self.seed)
+                for _, s in found:
+                    s['step'] = step
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the moments keep the types they were saved in (the base class casts them to the parameters')."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict['param_groups'] for i in g['params']]
+        params = [p for g in self.param_groups for p in g['params']]
+        for i, p in zip(ids, params):
+            saved = state_dict['state'].get(i)
+            if saved:
+                eight = saved['exp_avg'].dtype == CODES
+                _need(eight == (self.state_bits == 8), "AdamW: the saved moments have %d bits, this optimizer's %d", 8 if eight else 32, self.state_bits)
+                self.state[p] = {k: v.detach().to(p.device).clone() if isinstance(v, torch.Tensor) else v for k, v in saved.items()}
