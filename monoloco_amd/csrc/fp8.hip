@@ -10,6 +10,7 @@ using namespace mlk;
 namespace {
 
 constexpr long MAX_GRID = 0x7fffffffL;
+constexpr long G8_FROM256 = 256, G8_FROM128 = 256;
 
 int elem_size(int dtype) { return dtype == ML_F32 ? 4 : dtype == ML_BF16 || dtype == ML_F16 ? 2 : 0; }
 
@@ -44,6 +45,22 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
     else if (p.n <= 8192) rms_norm_back_kernel<T, 4, 4><<<g, 256, 0, s>>>(p);
     else if (p.n <= 32768) rms_norm_back_kernel<T, 16, 4><<<g, 1024, 0, s>>>(p);
     else rms_norm_back_kernel<T, 16, 0><<<g, 1024, 0, s>>>(p);
+}
+
+// Which product kernel: the ring wants rows that start on 16 bytes and offsets inside a tile below 2^32; its tile is the largest that
+// still gives every CU work.
+template <typename T>
+void launch_gemm(const GemmParams& p, unsigned grid64, hipStream_t s) {
+    const bool ring = p.fast_a && p.fast_b && p.lda < (1L << 23) && p.ldb < (1L << 23);
+    const long t256 = ((p.m + 255) / 256) * ((p.n + 255) / 256), t128 = ((p.m + 127) / 128) * ((p.n + 127) / 128);
+    const unsigned g16 = (unsigned)((p.n + 15) / 16);
+    if (p.m <= 16) fp8_gemm_rows_kernel<T, 1, 4><<<g16, 512, 0, s>>>(p);
+    else if (p.m <= 32) fp8_gemm_rows_kernel<T, 2, 2><<<g16, 512, 0, s>>>(p);
+    else if (p.m <= 64) fp8_gemm_rows_kernel<T, 4, 2><<<g16, 512, 0, s>>>(p);
+    else if (ring && sizeof(T) == 2 && t256 >= G8_FROM256) fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, (int)((p.m + 255) / 256), (int)((p.n + 255) / 256));
+    else if (ring && t128 >= G8_FROM128) fp8_gemm_ring_kernel<T, 2, 2><<<(unsigned)t128, 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
+    else if (ring) fp8_gemm_ring_kernel<T, 1, 1><<<grid64, 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
+    else fp8_gemm64_kernel<T><<<grid64, 256, 0, s>>>(p);
 }
 
 // workgroups of the backward pass = rows of its partial sums: enough to fill 256 CUs with 16 waves, few enough that writing and
@@ -103,7 +120,7 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
                  (long)m, (long)n, (long)k, (long)ldc, 0, 0, 0};
     p.fast_a = rows_aligned(a_dev, lda, 1, 16), p.fast_b = rows_aligned(b_dev, ldb, 1, 16), p.vec_c = rows_aligned(c_dev, ldc, es, 16);
     const hipStream_t s = (hipStream_t)stream;
-    with_type(c_dtype, [&](auto t) { fp8_gemm64_kernel<decltype(t)><<<(unsigned)grid, 256, 0, s>>>(p); });
+    with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, (unsigned)grid, s); });
     return ops_launched("ml_fp8_matmul");
 }
 

@@ -13,6 +13,8 @@
 // codes become bf16 in registers (exact: 4 significant bits; the scale is applied in the same conversion, exact as a power of two)
 // and v_mfma_f32_32x32x16_bf16 sums them -- half the rate, 4e-8 of the norm.
 #pragma once
+#include <type_traits>
+
 #include "block8.h"
 
 namespace mlk {
@@ -141,6 +143,330 @@ __global__ __launch_bounds__(256) void fp8_gemm64_kernel(GemmParams p) {
     for (int g = 0; g < 4; ++g) {
         const float v[4] = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
         store4<T>(p, m0 + wm * 32 + lr, n0 + wn * 32 + 8 * g + 4 * lh, v);
+    }
+}
+
+// ---- the ring kernel: (64 NJ) x (64 NI) of c per workgroup of 4 waves, 32 NJ x 32 NI per wave -----------------------------------
+// One wave per SIMD with 4 x 4 matrix tiles (256 accumulators) for large products, 2 x 2 and 1 x 1 (two and four workgroups per CU)
+// where the large tiles would be fewer than the CUs.  K runs in steps of 64 through a ring of four LDS slots (rows of 64 bytes, b then a)
+// that is filled by LDS-DMA four steps ahead: while step s multiplies, the fragments of s + 1 move into the other register set,
+// s + 2 and s + 3 are on their way, and s + 4 is requested into the slot whose fragments were read during s - 1.  One barrier per step;
+// the wait in front of it is counted (vmcnt(2 groups): s + 1 has landed).  The compiler does not know the DMA's instructions (inline
+// asm without outputs), so no ordinary vector load stands between the first request and the last wait except where a drain is meant
+// (the scales of the next 32 blocks).  The scales of 32 blocks of 128 for all rows of both operands lie in LDS behind the ring.
+// The last, partial block of 128 comes first, through registers, byte by byte where it must: pieces behind k become 0.
+// Rows behind m or n repeat the last one and are not stored.
+constexpr int G8_CHUNK = 32;              // blocks of 128 whose scales are in LDS at a time
+constexpr int G8_SPITCH = G8_CHUNK + 4;   // bytes per row of them: 32 rows fall into different banks
+
+template <typename T, int NI, int NJ>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 16 ? 1 : NI * NJ == 4 ? 2 : 4))) void fp8_gemm_ring_kernel(GemmParams p, int mt, int nt) {
+    constexpr int BN = 64 * NI, BM = 64 * NJ, ROWS = BN + BM, SLOT = ROWS * 64, RING = 4 * SLOT, NQ = NI + NJ;
+    __shared__ __attribute__((aligned(16))) char smem[RING + ROWS * G8_SPITCH];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wn = w & 1, wm = w >> 1;
+    const int ml = lane & 31, hh = lane >> 5;
+
+    // workgroup -> tile: consecutive workgroups go round the 8 XCDs; each XCD takes a contiguous run of tiles, in groups of 4 rows of
+    // tiles walked column by column, so that the tiles it works on at a time share operands in its L2
+    const int tiles = mt * nt, q8 = tiles >> 3, r8 = tiles & 7, xcd = blockIdx.x & 7;
+    const int tile = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
+    const int grp = tile / (4 * nt), rem = tile - grp * 4 * nt, gm = min(4, mt - grp * 4);
+    const long m0 = (long)(grp * 4 + rem % gm) * BM, n0 = (long)(rem / gm) * BN;
+
+    const int nkb = (int)(p.k / QB);                  // whole blocks of 128
+    const int nst = 2 * nkb;                          // steps of 64 in the ring
+    // ---- DMA: instruction q of this wave fetches 16 rows x 64 bytes; lane = row * 4 + piece, LDS linear, bank swizzle on the source
+    unsigned goff[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const bool isb = q < NI;
+        const int r = (isb ? (w * NI + q) : (w * NJ + q - NI)) * 16 + (lane >> 2);
+        const long last = (isb ? p.n - n0 : p.m - m0) - 1;
+        goff[q] = (unsigned)(min((long)r, last) * (isb ? p.ldb : p.lda)) + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
+    }
+    const uint8_t* rqb = p.b + n0 * p.ldb;   // the next step's first row of each operand (wave-uniform)
+    const uint8_t* rqa = p.a + m0 * p.lda;
+    const int lds0 = (int)(size_t)(__attribute__((address_space(3))) char*)smem;
+    auto request = [&](int slot, int q) {
+        const int at = lds0 + slot * SLOT + (q < NI ? (w * NI + q) * 1024 : BN * 64 + (w * NJ + q - NI) * 1024);
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(goff[q]), "s"(q < NI ? rqb : rqa), "s"(at) : "memory");
+    };
+
+    // ---- fragments: row (lane & 31) of a 32-row tile, two 16-byte pieces of its 64 (the same two of both operands)
+    const int swz = (ml >> 2) & 3;
+    const int boff = (wn * 32 * NI + ml) * 64, aoff = BN * 64 + (wm * 32 * NJ + ml) * 64;
+    const int c0 = (hh ^ swz) * 16, c1 = ((2 + hh) ^ swz) * 16;
+    struct Frag { i32x8 b[NI], a[NJ]; };
+    auto join = [](u32x4 x, u32x4 y) { return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]}; };
+    auto read_one = [&](Frag& f, const char* slot, int q) {
+        if (q < NI) f.b[q] = join(*(const u32x4*)(slot + boff + q * 2048 + c0), *(const u32x4*)(slot + boff + q * 2048 + c1));
+        else f.a[q - NI] = join(*(const u32x4*)(slot + aoff + (q - NI) * 2048 + c0), *(const u32x4*)(slot + aoff + (q - NI) * 2048 + c1));
+    };
+    // scale bytes of this lane's rows
+    unsigned sb[NI], sa[NJ], sbn[NI], san[NJ];
+    char* const slds = smem + RING;
+    auto read_scales = [&](int kb) {
+        const char* const at = slds + (kb & (G8_CHUNK - 1));
+#pragma unroll
+        for (int i = 0; i < NI; ++i) sbn[i] = *(const uint8_t*)(at + (wn * 32 * NI + i * 32 + ml) * G8_SPITCH);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) san[j] = *(const uint8_t*)(at + (BN + wm * 32 * NJ + j * 32 + ml) * G8_SPITCH);
+    };
+    auto scale_row = [&](int r) {   // r < BN: of b, else of a
+        if (r < BN) {
+            const long row = min(n0 + r, p.n - 1);
+            return p.sb + (p.b_tile ? row / QB : row) * p.ldsb;
+        }
+        const long row = min(m0 + r - BN, p.m - 1);
+        return p.sa + (p.a_tile ? row / QB : row) * p.ldsa;
+    };
+    auto fill_scales = [&](int kb0) {   // blocks kb0 .. kb0 + 31 of the whole ones
+        for (int u = tid; u < ROWS * (G8_CHUNK / 4); u += 256) {
+            const int r = u / (G8_CHUNK / 4), j = kb0 + (u % (G8_CHUNK / 4)) * 4;
+            if (j < nkb) {
+                const uint8_t* const src = scale_row(r) + j;
+                unsigned v = 0;
+                if (j + 4 <= nkb) {
+                    __builtin_memcpy(&v, src, 4);
+                } else {
+                    for (int e = 0; e < 4; ++e)
+                        if (j + e < nkb) v |= (unsigned)src[e] << (8 * e);
+                }
+                *(unsigned*)(slds + r * G8_SPITCH + (j - kb0)) = v;
+            }
+        }
+    };
+
+    f32x16 acc[NI][NJ];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x16{};
+
+    // one step's products (with fp32 results: through bf16, the codes of one 16-wide k piece at a time)
+    auto mul_row = [&](const Frag& f, int i) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mfma64<T>(f.b[i], f.a[j], acc[i][j], sb[i], sa[j]);
+    };
+
+    Frag f0, f1;
+    if (p.k > (long)nkb * QB) {   // the partial block
+        const long k0 = (long)nkb * QB;
+        for (int u = tid; u < ROWS * 8; u += 256) {
+            const int half = u / (ROWS * 4), v = u - half * ROWS * 4, r = v >> 2, ch = v & 3;
+            const long col = k0 + half * 64 + ch * 16;
+            const u32x4 x = r < BN ? load16(p.b, p.ldb, p.n, p.k, true, n0 + r, col) : load16(p.a, p.lda, p.m, p.k, true, m0 + r - BN, col);
+            *(u32x4*)(smem + half * SLOT + r * 64 + ((ch ^ ((r >> 2) & 3)) * 16)) = x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NI; ++i) sb[i] = scale_row(wn * 32 * NI + i * 32 + ml)[nkb];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) sa[j] = scale_row(BN + wm * 32 * NJ + j * 32 + ml)[nkb];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) read_one(f0, smem + half * SLOT, q);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) mul_row(f0, i);
+        }
+        __syncthreads();
+    }
+
+    if (nst > 0) {
+        fill_scales(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+            if (st < nst) {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) request(st, q);
+                rqb += 64, rqa += 64;
+                asm volatile("s_nop 4" ::: "memory");
+            }
+        }
+        // step 0 has landed (2 blocks = 4 steps are in flight, or 2)
+        if (nst > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NQ) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NQ) : "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) read_one(f0, smem, q);
+        read_scales(0);
+
+        // One step with the fragments FH; FN receives those of s + 1 (behind the last step: stale ones that nothing uses).  ODD: second
+        // half of a block, the next block's scales are read.  WAIT: requests that may be outstanding (-1: no wait).  No branch inside:
+        // the compiler would move the products behind it.
+        auto step = [&](int s, Frag& FH, Frag& FN, auto odd, auto request4, auto wait) {
+            constexpr bool ODD = decltype(odd)::value, MORE = decltype(request4)::value;
+            constexpr int WAIT = decltype(wait)::value;
+            if constexpr (WAIT >= 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(WAIT < 0 ? 0 : WAIT) : "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!ODD) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i) sb[i] = sbn[i];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) sa[j] = san[j];
+            }
+            const char* const next = smem + ((s + 1) & 3) * SLOT;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                mul_row(FH, i);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int q = i * NQ / NI; q < (i + 1) * NQ / NI; ++q) {
+                    if constexpr (MORE) request(s & 3, q);
+                    read_one(FN, next, q);
+                }
+                if (ODD && i == NI - 1) read_scales((s + 1) >> 1);
+            }
+            if constexpr (MORE) rqb += 64, rqa += 64;
+        };
+        auto chunk = [&](int s) {   // in front of the first step of the next 32 blocks: nobody reads the last ones' scales any more
+            if ((s & (2 * G8_CHUNK - 1)) == 0 && s > 0) {
+                fill_scales(s >> 1);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                read_scales(s >> 1);
+            }
+        };
+        constexpr std::integral_constant<bool, false> no{};
+        constexpr std::integral_constant<bool, true> yes{};
+        constexpr std::integral_constant<int, 2 * NQ> two{};
+        constexpr std::integral_constant<int, NQ> one{};
+        constexpr std::integral_constant<int, 0> all{};
+        constexpr std::integral_constant<int, -1> none{};
+        int s = 0;
+#pragma clang loop unroll(disable)
+        for (; s < nst - 4; s += 2) {
+            chunk(s);
+            step(s, f0, f1, no, yes, two);
+            step(s + 1, f1, f0, yes, yes, two);
+        }
+        if (s < nst - 2) {
+            chunk(s);
+            step(s, f0, f1, no, no, two);
+            step(s + 1, f1, f0, yes, no, one);
+            s += 2;
+        }
+        chunk(s);
+        step(s, f0, f1, no, no, all);
+        step(s + 1, f1, f0, yes, no, none);
+    }
+
+    // ---- epilogue: 32 rows of c x this wave's 32 NI columns at a time through LDS (the ring is idle), then whole rows
+    __syncthreads();
+    constexpr int ROWB = 32 * NI * (int)sizeof(T), PITCH = ROWB + 16, PIECES = ROWB / 16;
+    static_assert(BN <= 256 && 4 * 32 * PITCH + BN * 4 <= RING + ROWS * G8_SPITCH, "epilogue scratch");
+    char* const scr = smem + w * 32 * PITCH;
+    float* const bias = (float*)(smem + 4 * 32 * PITCH);   // this workgroup's columns
+    if (tid < BN) bias[tid] = bias_at(p, n0 + tid);
+    __syncthreads();
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = i * 32 + 8 * g + 4 * hh;
+                const f32x4 b4 = *(const f32x4*)(bias + wn * 32 * NI + col);
+                t4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j][4 * g + e] + b4[e]);
+                *(t4*)(scr + ml * PITCH + col * (int)sizeof(T)) = v;
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wave's own scratch: no barrier)
+#pragma unroll
+        for (int u = 0; u < 32 * PIECES / 64; ++u) {
+            const int at = u * 64 + lane, r = at / PIECES, c = at % PIECES;
+            const long row = m0 + wm * 32 * NJ + j * 32 + r, col = n0 + wn * 32 * NI + c * (16 / (int)sizeof(T));
+            const tv v = *(const tv*)(scr + r * PITCH + c * 16);
+            if (row < p.m && col < p.n) {
+                T* const out = (T*)p.c + row * p.ldc + col;
+                if (p.vec_c && col + 16 / (int)sizeof(T) <= p.n) {
+                    *(tv*)out = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+                        if (col + e < p.n) out[e] = v[e];
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// ---- few rows of a: 16 MT x 16 of c per workgroup of 8 waves, which share the blocks of k --------------------------------------
+// Bound by reading b once (for one row: 16 MB of a 4096 x 4096 weight), so every CU pulls on it: n / 16 workgroups, each wave takes every
+// eighth block of 128 straight into fragments (16 rows x 128 contiguous bytes per load pair, no LDS), U blocks in flight; the eight partial
+// results meet in LDS in a fixed order.  Right for every stride and alignment.
+template <typename T>
+__device__ __forceinline__ f32x4 mfma128(i32x8 a, i32x8 b, f32x4 c, unsigned sa, unsigned sb) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(a[2 * s], a[2 * s + 1], sa), to_bf16(b[2 * s], b[2 * s + 1], sb), c, 0, 0, 0);
+        return c;
+    } else {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
+    }
+}
+
+template <typename T, int MT, int U>
+__global__ __launch_bounds__(512) void fp8_gemm_rows_kernel(GemmParams p) {
+    constexpr int WAVES = 8;
+    __shared__ __attribute__((aligned(16))) float part[WAVES][MT][64][4];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+    const long n0 = (long)blockIdx.x * 16, kb = (p.k + QB - 1) / QB;
+    const long brow = min(n0 + lr, p.n - 1);
+    const uint8_t* const sb = p.sb + (p.b_tile ? brow / QB : brow) * p.ldsb;
+    const uint8_t* sa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const long r = min((long)(i * 16 + lr), p.m - 1);
+        sa[i] = p.sa + (p.a_tile ? r / QB : r) * p.ldsa;
+    }
+    auto frag = [&](const uint8_t* x, long ld, long rows, bool fast, long row, long col) {
+        const u32x4 u = load16(x, ld, rows, p.k, fast, row, col), v = load16(x, ld, rows, p.k, fast, row, col + 16);
+        return i32x8{(int)u[0], (int)u[1], (int)u[2], (int)u[3], (int)v[0], (int)v[1], (int)v[2], (int)v[3]};
+    };
+    f32x4 acc[MT] = {};
+    for (long t = w; t < kb; t += WAVES * U) {
+        i32x8 fb[U], fa[U][MT];
+        unsigned xb[U], xa[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long b = t + u * WAVES, col = b * QB + lg * 32;    // (behind the last block: zeros, scale 1)
+            fb[u] = frag(p.b, p.ldb, p.n, p.fast_b, n0 + lr, col);
+            xb[u] = b < kb ? sb[b] : 127;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                fa[u][i] = frag(p.a, p.lda, p.m, p.fast_a, i * 16 + lr, col);
+                xa[u][i] = b < kb ? sa[i][b] : 127;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] = mfma128<T>(fb[u], fa[u][i], acc[i], xb[u], xa[u][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *(f32x4*)part[w][i][lane] = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < MT * 256; e += 512) {    // element (row i * 16 + r, column c): neighbouring threads, neighbouring columns
+        const int c = e & 15, r = (e >> 4) & 15, i = e >> 8;
+        const long row = i * 16 + r, col = n0 + c;
+        if (row >= p.m || col >= p.n) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) v += part[x][i][(c >> 2) * 16 + r][c & 3];
+        ((T*)p.c)[row * p.ldc + col] = (T)(v + bias_at(p, col));
     }
 }
 
