@@ -441,6 +441,17 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
 int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
                   const uint8_t* b_scale_dev, int64_t ldsb, int b_tile, const void* bias_dev, int bias_dtype, void* c_dev, int c_dtype,
                   int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream);
+/* A linear layer with both operands in 8 bits, forward and backward, each in one call: y (m, n) = Q(x) . Q(w)^T [+ bias], x (m, k) in 1 x 128
+ * blocks, w (n, k) in tiles, y of x's type; dx = Q(dy) . Q(w); dw = Q(dy^T) . Q(x^T)^T, 1 x 128 blocks along the batch; db = column sums of
+ * dy.  bytes3 = {forward's workspace, what backward needs (kept by the caller between the two calls), backward's workspace}, all aligned to
+ * 256 bytes; need_dx / need_dw: the same in all three calls.  dx_dev, dw_dev, db_dev may be NULL; they are contiguous, of their own types. */
+int ml_fp8_linear_sizes(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, int need_db, int64_t* bytes3);
+int ml_fp8_linear(const void* x_dev, int x_dtype, int64_t ldx, const void* w_dev, int w_dtype, int64_t ldw, const void* bias_dev,
+                  int bias_dtype, void* y_dev, int64_t ldy, int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, void* work_dev,
+                  void* saved_dev, void* stream);
+int ml_fp8_linear_backward(const void* dy_dev, int dy_dtype, int64_t ldy, const void* saved_dev, void* dx_dev, int dx_dtype, void* dw_dev,
+                           int dw_dtype, void* db_dev, int db_dtype, int64_t m, int64_t n, int64_t k, int need_dx, int need_dw,
+                           void* work_dev, void* stream);
 /* h = x [+ residual]; y = h / sqrt(mean(h^2) + eps) * w over rows of n.  x, residual, h, y of `dtype`; w (n) of `dtype` or fp32.  Exactly one
  * of y_dev and q_dev (+ scale_dev: y as 1 x 128 blocks of codes) is written; h_dev may be NULL.  y and the row statistics come from h
  * before its rounding to `dtype`. */

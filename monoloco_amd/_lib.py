@@ -126,6 +126,11 @@ SIGNATURES = {
     'ml_fp8_quantize': (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P]),
     'ml_fp8_matmul': (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int64, _P, c_int64, c_int, _P, c_int, _P, c_int, c_int64, c_int64,
                               c_int64, c_int64, _P]),
+    'ml_fp8_linear_sizes': (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_int, _P]),
+    'ml_fp8_linear': (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, c_int, _P, c_int64, c_int64, c_int64, c_int64, c_int, c_int, _P,
+                              _P, _P]),
+    'ml_fp8_linear_backward': (c_int, [_P, c_int, c_int64, _P, _P, c_int, _P, c_int, _P, c_int, c_int64, c_int64, c_int64, c_int, c_int,
+                                       _P, _P]),
     'ml_rms_norm': (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int, c_int64, c_int64, c_float, _P, c_int64, _P, c_int64, _P, c_int64,
                             _P, c_int64, _P]),
     'ml_rms_norm_backward_groups': (c_int64, [c_int64, c_int64]),

@@ -71,6 +71,19 @@ long norm_groups(long m, long n) {
     return g < most ? g : most;
 }
 
+// the bias gradient alone: the tile kernel without either form of codes
+int column_sums(const void* x, int dtype, int64_t m, int64_t n, int64_t ldx, float* out, hipStream_t s) {
+    const int es = elem_size(dtype);
+    if (!es || (m && n && ldx < n)) return ops_fail(ML_ERR_ARG, "column sums: bad type %d or row stride", dtype);
+    if (m == 0 || n == 0) return ML_OK;
+    QuantParams p{};
+    p.x = x, p.m = m, p.n = n, p.ldx = ldx, p.colsum = out, p.vec = rows_aligned(x, ldx, es, 16);
+    const long grid = ((n + QB - 1) / QB) * ((m + QB - 1) / QB);
+    if (grid > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "column sums: %lld x %lld is too large", (long long)m, (long long)n);
+    with_type(dtype, [&](auto t) { quantize_tile_kernel<decltype(t)><<<(unsigned)grid, 256, 0, s>>>(p); });
+    return ops_launched("column sums");
+}
+
 }  // namespace
 
 extern "C" {
@@ -122,6 +135,75 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
     const hipStream_t s = (hipStream_t)stream;
     with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, (unsigned)grid, s); });
     return ops_launched("ml_fp8_matmul");
+}
+
+// ---- a linear layer in one call: buffers at multiples of 256 bytes inside two workspaces
+static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+namespace {
+struct LinearPlan {
+    int64_t kb, nb, mb, ldk, ldn, ldm;                  // blocks; row strides of codes along k, n, m
+    int64_t qx, sx, qw, sw, forward;                    // forward's workspace
+    int64_t qxt, sxt, qwt, swt, saved;                  // what the backward pass needs
+    int64_t qd, sd, qdt, sdt, part, backward;           // backward's workspace
+    LinearPlan(int64_t m, int64_t n, int64_t k, bool need_dx, bool need_dw, bool need_db) {
+        kb = (k + QB - 1) / QB, nb = (n + QB - 1) / QB, mb = (m + QB - 1) / QB;
+        ldk = round_up(k, 16), ldn = round_up(n, 16), ldm = round_up(m, 16);
+        int64_t at = 0;
+        auto take = [&](int64_t bytes) { const int64_t r = at; at += round_up(bytes, 256); return r; };
+        qx = take(m * ldk), sx = take(m * kb), qw = take(n * ldk), sw = take(nb * kb), forward = at;
+        at = 0;
+        qxt = take(need_dw ? k * ldm : 0), sxt = take(need_dw ? k * mb : 0);
+        qwt = take(need_dx ? k * ldn : 0), swt = take(need_dx ? kb * nb : 0), saved = at;
+        at = 0;
+        qd = take(need_dx ? m * ldn : 0), sd = take(need_dx ? m * nb : 0);
+        qdt = take(need_dw ? n * ldm : 0), sdt = take(need_dw ? n * mb : 0);
+        part = take(need_db ? mb * n * 4 : 0), backward = at;
+    }
+};
+}  // namespace
+
+int ml_fp8_linear_sizes(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, int need_db, int64_t* bytes3) {
+    if (m < 0 || n < 0 || k < 0 || m > (1LL << 40) || n > (1LL << 40) || k > (1LL << 40) || !bytes3) return ops_fail(ML_ERR_ARG, "ml_fp8_linear_sizes: bad size or null pointer");
+    const LinearPlan l(m, n, k, need_dx, need_dw, need_db);
+    bytes3[0] = l.forward, bytes3[1] = l.saved, bytes3[2] = l.backward;
+    return ML_OK;
+}
+
+int ml_fp8_linear(const void* x_dev, int x_dtype, int64_t ldx, const void* w_dev, int w_dtype, int64_t ldw, const void* bias_dev, int bias_dtype, void* y_dev,
+                  int64_t ldy, int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, void* work_dev, void* saved_dev, void* stream) {
+    if (m < 0 || n < 0 || k < 1) return ops_fail(ML_ERR_ARG, "ml_fp8_linear: bad size");
+    if ((m && n && !work_dev) || ((need_dx || need_dw) && n && !saved_dev)) return ops_fail(ML_ERR_ARG, "ml_fp8_linear: null workspace");
+    const LinearPlan l(m, n, k, need_dx, need_dw, false);
+    uint8_t *const wk = (uint8_t*)work_dev, *const sv = (uint8_t*)saved_dev;
+    int rc = ml_fp8_quantize(x_dev, x_dtype, m, k, ldx, 0, wk + l.qx, l.ldk, wk + l.sx, l.kb, need_dw ? sv + l.qxt : nullptr, l.ldm, need_dw ? sv + l.sxt : nullptr,
+                             l.mb, nullptr, stream);
+    if (!rc)
+        rc = ml_fp8_quantize(w_dev, w_dtype, n, k, ldw, 1, wk + l.qw, l.ldk, wk + l.sw, l.kb, need_dx ? sv + l.qwt : nullptr, l.ldn, need_dx ? sv + l.swt : nullptr,
+                             l.nb, nullptr, stream);
+    if (!rc) rc = ml_fp8_matmul(wk + l.qx, l.ldk, wk + l.sx, l.kb, 0, wk + l.qw, l.ldk, wk + l.sw, l.kb, 1, bias_dev, bias_dtype, y_dev, x_dtype, ldy, m, n, k, stream);
+    return rc;
+}
+
+int ml_fp8_linear_backward(const void* dy_dev, int dy_dtype, int64_t ldy, const void* saved_dev, void* dx_dev, int dx_dtype, void* dw_dev, int dw_dtype, void* db_dev,
+                           int db_dtype, int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, void* work_dev, void* stream) {
+    if (m < 0 || n < 0 || k < 1) return ops_fail(ML_ERR_ARG, "ml_fp8_linear_backward: bad size");
+    // (the layout of `saved` goes by what the forward pass was asked for, the work by what is asked for now)
+    const LinearPlan l(m, n, k, need_dx, need_dw, db_dev != nullptr);
+    const bool dx = dx_dev != nullptr, dw = dw_dev != nullptr;
+    if ((dx && !need_dx) || (dw && !need_dw)) return ops_fail(ML_ERR_ARG, "ml_fp8_linear_backward: a gradient that the forward pass did not prepare");
+    if (m && n && (!dy_dev || !work_dev || ((dx || dw) && !saved_dev))) return ops_fail(ML_ERR_ARG, "ml_fp8_linear_backward: null pointer");
+    uint8_t *const wk = (uint8_t*)work_dev, *const sv = (uint8_t*)saved_dev;
+    int rc = 0;
+    if (dx || dw)
+        rc = ml_fp8_quantize(dy_dev, dy_dtype, m, n, ldy, 0, dx ? wk + l.qd : nullptr, l.ldn, dx ? wk + l.sd : nullptr, l.nb, dw ? wk + l.qdt : nullptr, l.ldm,
+                             dw ? wk + l.sdt : nullptr, l.mb, db_dev ? (float*)(wk + l.part) : nullptr, stream);
+    else if (db_dev)
+        rc = column_sums(dy_dev, dy_dtype, m, n, ldy, (float*)(wk + l.part), (hipStream_t)stream);
+    if (!rc && dx) rc = ml_fp8_matmul(wk + l.qd, l.ldn, wk + l.sd, l.nb, 0, sv + l.qwt, l.ldn, sv + l.swt, l.nb, 1, nullptr, 0, dx_dev, dx_dtype, k, m, k, n, stream);
+    if (!rc && dw) rc = ml_fp8_matmul(wk + l.qdt, l.ldm, wk + l.sdt, l.mb, 0, sv + l.qxt, l.ldm, sv + l.sxt, l.mb, 0, nullptr, 0, dw_dev, dw_dtype, k, n, k, m, stream);
+    if (!rc && db_dev) rc = ml_sum_rows((const float*)(wk + l.part), m ? l.mb : 0, n, db_dev, db_dtype, stream);
+    return rc;
 }
 
 int ml_rms_norm(const void* x_dev, int64_t ldx, const void* residual_dev, int64_t ldr, int dtype, const void* w_dev, int w_dtype, int64_t m,

@@ -2,18 +2,21 @@
 
 For the loop a caller owns (``outputs = model(inputs)``; ``loss.backward()``; ``optimizer.step()``): the reference builds torch's Adam
 there (monoloco/train/trainer.py:128-131).  ``HipTrainer`` has its own Adam inside the library and does not need this one."""
-import ctypes
+from array import array
+from operator import attrgetter
 
 import torch
 
 from .. import _lib
-from .._lib import MonolocoHipError, check_ops
-from ..engine import _stream
-from ..fp8 import BLOCK, CODES, DTYPES, SCALES, _need
+from .._lib import MonolocoHipError
+from ..fp8 import BLOCK, CODES, DTYPES, SCALES, _need, _run
+
+_T = torch.Tensor
+_dtype = attrgetter('dtype')
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+def _address(a):
+    return a.buffer_info()[0]
 
 
 def state_scales(numel, device):
@@ -34,30 +37,39 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr=1e
     _need(int(step) >= 1, "adamw_step: steps are counted from 1, got %r", step)
     if not k:
         return
-    dev, dt = params[0].device, params[0].dtype
-    if dev.type != 'cuda':
-        raise MonolocoHipError("adamw_step runs on HIP devices only, got a tensor on %s (there is no CPU fallback)" % (dev,))
+    dt, index = params[0].dtype, params[0].get_device()
+    if not params[0].is_cuda:
+        raise MonolocoHipError("adamw_step runs on HIP devices only, got a tensor on %s (there is no CPU fallback)" % (params[0].device,))
     _need(dt in DTYPES, "adamw_step: parameters are fp32, bf16 or fp16, got %s", dt)
     mdt = torch.float32 if scales is None else CODES
-    sizes = [p.numel() for p in params]
-    for p, g, m, v, n in zip(params, grads, exp_avgs, exp_avg_sqs, sizes):
-        _need(p.dtype == dt and g.dtype == dt and m.dtype == mdt and v.dtype == mdt, "adamw_step: %s parameters take %s gradients and %s moments, got %s, %s, %s, %s",
-              dt, dt, mdt, p.dtype, g.dtype, m.dtype, v.dtype)
-        _need(p.device == dev and g.device == dev and m.device == dev and v.device == dev, "adamw_step: tensors on several devices")
-        _need(p.is_contiguous() and m.is_contiguous() and v.is_contiguous(), "adamw_step: parameters and moments have to be contiguous")
-        _need(g.numel() == n and m.numel() == n and v.numel() == n, "adamw_step: a gradient or moment of another size than its parameter")
+    # (whole lists at a time: for a network of 38 tensors a check per tensor and property costs more than the launch)
+    sizes = list(map(_T.numel, params))
+    for what, ts, want in (('parameters', params, dt), ('gradients', grads, dt), ('first moments', exp_avgs, mdt), ('second moments', exp_avg_sqs, mdt)):
+        if set(map(_dtype, ts)) != {want}:
+            raise ValueError("adamw_step: %s parameters take %s gradients and %s moments, got %s as %s" % (dt, dt, mdt, sorted(map(str, set(map(_dtype, ts)))), what))
+        if set(map(_T.get_device, ts)) != {index}:
+            raise ValueError("adamw_step: the %s are not all on cuda:%d" % (what, index))
+        if ts is not params and list(map(_T.numel, ts)) != sizes:
+            raise ValueError("adamw_step: the %s are not of their parameters' sizes" % what)
+        if not all(map(_T.is_contiguous, ts)):
+            if ts is not grads:
+                raise ValueError("adamw_step: the %s have to be contiguous" % what)
+            grads = [g.contiguous() for g in grads]
     if scales is not None:
         for s, n in zip(scales, sizes):
-            _need(s.dtype == SCALES and s.device == dev and s.is_contiguous() and tuple(s.shape) == (2, -(-n // BLOCK)),
-                  "adamw_step: the scales of %d elements are a contiguous (2, %d) of %s on %s, got %s %s", n, -(-n // BLOCK), SCALES, dev, tuple(s.shape), s.dtype)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    ps, gs, ms, vs = _pointers(params), _pointers(grads), _pointers(exp_avgs), _pointers(exp_avg_sqs)
-    written = [a for t in (ps, ms, vs) for a, n in zip(t, sizes) if n]
-    _need(len(set(written)) == len(written), "adamw_step: a tensor is given twice")
-    with torch.cuda.device(dev):
-        check_ops(_lib.load().ml_adamw_step(
-            k, (ctypes.c_int64 * k)(*sizes), ps, gs, DTYPES[dt], ms, vs, None if scales is None else _pointers(scales),
-            int(step), float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(seed) & 0xffffffff, _stream(dev)))
+            if not (s.dtype == SCALES and s.get_device() == index and s.is_contiguous() and tuple(s.shape) == (2, -(-n // BLOCK))):
+                raise ValueError("adamw_step: the scales of %d elements are a contiguous (2, %d) of %s on cuda:%d, got %s %s on %s"
+                                 % (n, -(-n // BLOCK), SCALES, index, tuple(s.shape), s.dtype, s.device))
+    ps, gs, ms, vs = (array('Q', map(_T.data_ptr, ts)) for ts in (params, grads, exp_avgs, exp_avg_sqs))
+    ss = array('Q', map(_T.data_ptr, scales)) if scales is not None else None
+    written = {*ps, *ms, *vs}
+    if len(written) != 3 * k:
+        written = [a for ts in (ps, ms, vs) for a, n in zip(ts, sizes) if n]
+        _need(len(set(written)) == len(written), "adamw_step: a tensor is given twice")
+    numel = array('q', sizes)
+    _run(index, _lib.load().ml_adamw_step, k, _address(numel), _address(ps), _address(gs),
+         DTYPES[dt], _address(ms), _address(vs), None if ss is None else _address(ss), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps),
+         float(weight_decay), int(seed) & 0xffffffff)
     torch.autograd.graph.increment_version(params)   # (LocoModel re-packs its engine when a parameter's version moved)
 
 
