@@ -162,7 +162,7 @@ constexpr int G8_SPITCH = G8_CHUNK + 4;   // bytes per row of them: 32 rows fall
 template <typename T, int NI, int NJ>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 16 ? 1 : NI * NJ == 4 ? 2 : 4))) void fp8_gemm_ring_kernel(GemmParams p, int mt, int nt) {
     constexpr int BN = 64 * NI, BM = 64 * NJ, ROWS = BN + BM, SLOT = ROWS * 64, RING = 4 * SLOT, NQ = NI + NJ;
-    __shared__ __attribute__((aligned(16))) char smem[RING + ROWS * G8_SPITCH];
+    __shared__ __attribute__((aligned(16))) char smem[RING + ROWS * G8_SPITCH + BN * 4];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wn = w & 1, wm = w >> 1;
     const int ml = lane & 31, hh = lane >> 5;
 
@@ -220,21 +220,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         const long row = min(m0 + r - BN, p.m - 1);
         return p.sa + (p.a_tile ? row / QB : row) * p.ldsa;
     };
-    auto fill_scales = [&](int kb0) {   // blocks kb0 .. kb0 + 31 of the whole ones
-        for (int u = tid; u < ROWS * (G8_CHUNK / 4); u += 256) {
-            const int r = u / (G8_CHUNK / 4), j = kb0 + (u % (G8_CHUNK / 4)) * 4;
-            if (j < nkb) {
-                const uint8_t* const src = scale_row(r) + j;
-                unsigned v = 0;
-                if (j + 4 <= nkb) {
-                    __builtin_memcpy(&v, src, 4);
+    // blocks kb0 .. kb0 + 31 of the whole ones; a thread takes whole rows and issues all its loads before the first wait (a loop of single
+    // loads cost 10 us in front of every tile)
+    auto fill_scales = [&](int kb0) {
+        constexpr int RT = (ROWS + 255) / 256;
+        unsigned v[RT][G8_CHUNK / 4];
+        const int have = min(nkb - kb0, G8_CHUNK);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int r = tid + 256 * i;
+            const uint8_t* const src = scale_row(r < ROWS ? r : 0) + kb0;
+#pragma unroll
+            for (int j = 0; j < G8_CHUNK / 4; ++j) {
+                v[i][j] = 0;
+                if (4 * j + 4 <= have) {
+                    __builtin_memcpy(&v[i][j], src + 4 * j, 4);
                 } else {
-                    for (int e = 0; e < 4; ++e)
-                        if (j + e < nkb) v |= (unsigned)src[e] << (8 * e);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (4 * j + e < have) v[i][j] |= (unsigned)src[4 * j + e] << (8 * e);
                 }
-                *(unsigned*)(slds + r * G8_SPITCH + (j - kb0)) = v;
             }
         }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < G8_CHUNK / 4; ++j)
+                if (tid + 256 * i < ROWS && 4 * j < have) *(unsigned*)(slds + (tid + 256 * i) * G8_SPITCH + 4 * j) = v[i][j];
     };
 
     f32x16 acc[NI][NJ];
@@ -273,9 +285,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         __syncthreads();
     }
 
+    float* const bias = (float*)(slds + ROWS * G8_SPITCH);   // this workgroup's columns
+    if (tid < BN) bias[tid] = bias_at(p, n0 + tid);
     if (nst > 0) {
-        fill_scales(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
@@ -286,9 +298,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
                 asm volatile("s_nop 4" ::: "memory");
             }
         }
-        // step 0 has landed (2 blocks = 4 steps are in flight, or 2)
-        if (nst > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NQ) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NQ) : "memory");
+        fill_scales(0);   // (its wait is the first steps', too: their latencies overlap)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -361,11 +372,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
     // ---- epilogue: 32 rows of c x this wave's 32 NI columns at a time through LDS (the ring is idle), then whole rows
     __syncthreads();
     constexpr int ROWB = 32 * NI * (int)sizeof(T), PITCH = ROWB + 16, PIECES = ROWB / 16;
-    static_assert(BN <= 256 && 4 * 32 * PITCH + BN * 4 <= RING + ROWS * G8_SPITCH, "epilogue scratch");
+    static_assert(BN <= 256 && 4 * 32 * PITCH <= RING, "epilogue scratch");
     char* const scr = smem + w * 32 * PITCH;
-    float* const bias = (float*)(smem + 4 * 32 * PITCH);   // this workgroup's columns
-    if (tid < BN) bias[tid] = bias_at(p, n0 + tid);
-    __syncthreads();
     typedef T t4 __attribute__((ext_vector_type(4)));
     typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
 #pragma unroll
