@@ -286,7 +286,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
     }
 
     float* const bias = (float*)(slds + ROWS * G8_SPITCH);   // this workgroup's columns
-    if (tid < BN) bias[tid] = bias_at(p, n0 + tid);
     if (nst > 0) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -298,7 +297,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
                 asm volatile("s_nop 4" ::: "memory");
             }
         }
+        const float b = tid < BN ? bias_at(p, n0 + tid) : 0.0f;
         fill_scales(0);   // (its wait is the first steps', too: their latencies overlap)
+        if (tid < BN) bias[tid] = b;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
@@ -323,17 +324,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
                 for (int j = 0; j < NJ; ++j) sa[j] = san[j];
             }
             const char* const next = smem + ((s + 1) & 3) * SLOT;
+            // requests and reads behind the first half of the products: the second half covers the last reads' latency in front of the
+            // next barrier (spread over all of them, every step waited ~400 of its 1440 cycles there)
+            constexpr int NM = NI * NJ, HALF = NM > 1 ? NM / 2 : 1;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
+            for (int x = 0; x < NM; ++x) {
+                const int i = x / NJ, j = x % NJ;
                 __builtin_amdgcn_sched_barrier(0);
-                mul_row(FH, i);
+                acc[i][j] = mfma64<T>(FH.b[i], FH.a[j], acc[i][j], sb[i], sa[j]);
                 __builtin_amdgcn_sched_barrier(0);
+                if (x < HALF) {
 #pragma unroll
-                for (int q = i * NQ / NI; q < (i + 1) * NQ / NI; ++q) {
-                    if constexpr (MORE) request(s & 3, q);
-                    read_one(FN, next, q);
+                    for (int q = x * NQ / HALF; q < (x + 1) * NQ / HALF; ++q) {
+                        if constexpr (MORE) request(s & 3, q);
+                        read_one(FN, next, q);
+                    }
+                    if (ODD && x == HALF - 1) read_scales((s + 1) >> 1);
                 }
-                if (ODD && i == NI - 1) read_scales((s + 1) >> 1);
             }
             if constexpr (MORE) rqb += 64, rqa += 64;
         };
@@ -367,42 +374,72 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         chunk(s);
         step(s, f0, f1, no, no, all);
         step(s + 1, f1, f0, yes, no, none);
+    } else if (tid < BN) {
+        bias[tid] = bias_at(p, n0 + tid);
     }
 
-    // ---- epilogue: 32 rows of c x this wave's 32 NI columns at a time through LDS (the ring is idle), then whole rows
+    // ---- epilogue: this wave's rows of c through LDS (the ring and the scales are done with), then whole rows with 16-byte stores.
+    // PASS matrix tiles along m at a time, as many as fit; a tile inside c takes straight-line code, eight stores in flight.
     __syncthreads();
-    constexpr int ROWB = 32 * NI * (int)sizeof(T), PITCH = ROWB + 16, PIECES = ROWB / 16;
-    static_assert(BN <= 256 && 4 * 32 * PITCH <= RING, "epilogue scratch");
-    char* const scr = smem + w * 32 * PITCH;
+    constexpr int ES = (int)sizeof(T), ROWB = 32 * NI * ES, PITCH = ROWB + 16, PIECES = ROWB / 16, EV = 16 / ES;
+    constexpr int PASS = NJ * 4 * 32 * PITCH <= RING + ROWS * G8_SPITCH ? NJ : NJ / 2;
+    static_assert(BN <= 256 && PASS * 4 * 32 * PITCH <= RING + ROWS * G8_SPITCH, "epilogue scratch");
+    char* const scr = smem + w * PASS * 32 * PITCH;
     typedef T t4 __attribute__((ext_vector_type(4)));
-    typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
+    typedef T tv __attribute__((ext_vector_type(EV)));
+    const bool inside = m0 + BM <= p.m && n0 + BN <= p.n && p.vec_c;
+    const long row0 = m0 + wm * 32 * NJ, col0 = n0 + wn * 32 * NI;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
+    for (int j0 = 0; j0 < NJ; j0 += PASS) {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int col = i * 32 + 8 * g + 4 * hh;
                 const f32x4 b4 = *(const f32x4*)(bias + wn * 32 * NI + col);
-                t4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j][4 * g + e] + b4[e]);
-                *(t4*)(scr + ml * PITCH + col * (int)sizeof(T)) = v;
+                for (int j = 0; j < PASS; ++j) {
+                    t4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j0 + j][4 * g + e] + b4[e]);
+                    *(t4*)(scr + (j * 32 + ml) * PITCH + col * ES) = v;
+                }
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wave's own scratch: no barrier)
+        constexpr int UNITS = PASS * 32 * PIECES / 64, STEP = 64 / PIECES;   // a unit: STEP rows
+        const int r = lane / PIECES, c = lane % PIECES;
+        const char* const from = scr + r * PITCH + c * 16;
+        if (inside) {
+            T* out = (T*)p.c + (row0 + j0 * 32 + r) * p.ldc + col0 + c * EV;
+            const long by = (long)STEP * p.ldc;
 #pragma unroll
-        for (int u = 0; u < 32 * PIECES / 64; ++u) {
-            const int at = u * 64 + lane, r = at / PIECES, c = at % PIECES;
-            const long row = m0 + wm * 32 * NJ + j * 32 + r, col = n0 + wn * 32 * NI + c * (16 / (int)sizeof(T));
-            const tv v = *(const tv*)(scr + r * PITCH + c * 16);
-            if (row < p.m && col < p.n) {
-                T* const out = (T*)p.c + row * p.ldc + col;
-                if (p.vec_c && col + 16 / (int)sizeof(T) <= p.n) {
-                    *(tv*)out = v;
-                } else {
+            for (int u = 0; u < UNITS; u += 8) {
+                tv v[8];
 #pragma unroll
-                    for (int e = 0; e < 16 / (int)sizeof(T); ++e)
-                        if (col + e < p.n) out[e] = v[e];
+                for (int x = 0; x < 8; ++x)
+                    if (u + x < UNITS) v[x] = *(const tv*)(from + (u + x) * STEP * PITCH);
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    if (u + x < UNITS) {
+                        *(tv*)out = v[x];
+                        out += by;
+                    }
+            }
+        } else {
+            const long col = col0 + c * EV;
+#pragma clang loop unroll(disable)
+            for (int u = 0; u < UNITS; ++u) {
+                const long row = row0 + j0 * 32 + r + u * STEP;
+                const tv v = *(const tv*)(from + u * STEP * PITCH);
+                if (row < p.m && col < p.n) {
+                    T* const out = (T*)p.c + row * p.ldc + col;
+                    if (p.vec_c && col + EV <= p.n) {
+                        *(tv*)out = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < EV; ++e)
+                            if (col + e < p.n) out[e] = v[e];
+                    }
                 }
             }
         }
