@@ -57,7 +57,9 @@ void launch_gemm(const GemmParams& p, unsigned grid64, hipStream_t s) {
     if (p.m <= 16) fp8_gemm_rows_kernel<T, 1, 4><<<g16, 512, 0, s>>>(p);
     else if (p.m <= 32) fp8_gemm_rows_kernel<T, 2, 2><<<g16, 512, 0, s>>>(p);
     else if (p.m <= 64) fp8_gemm_rows_kernel<T, 4, 2><<<g16, 512, 0, s>>>(p);
-    else if (ring && sizeof(T) == 2 && t256 >= G8_FROM256) fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, (int)((p.m + 255) / 256), (int)((p.n + 255) / 256));
+    else if (ring && sizeof(T) == 2 && t256 >= G8_FROM256 && p.k % QB == 0 && p.k >= 512 && p.n % 8 == 0 && p.vec_c) {
+        if constexpr (sizeof(T) == 2) fp8_gemm_stream_kernel<T><<<(unsigned)(t256 < 256 ? t256 : 256), 256, 0, s>>>(p, (int)((p.m + 255) / 256), (int)((p.n + 255) / 256));
+    } else if (ring && sizeof(T) == 2 && t256 >= G8_FROM256) fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, (int)((p.m + 255) / 256), (int)((p.n + 255) / 256));
     else if (ring && t128 >= G8_FROM128) fp8_gemm_ring_kernel<T, 2, 2><<<(unsigned)t128, 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
     else if (ring) fp8_gemm_ring_kernel<T, 1, 1><<<grid64, 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
     else fp8_gemm64_kernel<T><<<grid64, 256, 0, s>>>(p);

@@ -157,6 +157,7 @@ __global__ __launch_bounds__(256) void fp8_gemm64_kernel(GemmParams p) {
 // The last, partial block of 128 comes first, through registers, byte by byte where it must: pieces behind k become 0.
 // Rows behind m or n repeat the last one and are not stored.
 constexpr int G8_CHUNK = 32;              // blocks of 128 whose scales are in LDS at a time
+constexpr int G8_REQ0 = 8;               // streaming kernel: the product of a step behind which its requests begin
 constexpr int G8_SPITCH = G8_CHUNK + 4;   // bytes per row of them: 32 rows fall into different banks
 
 template <typename T, int NI, int NJ>
@@ -445,6 +446,234 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+}
+
+// one accumulator, AGPR -> VGPR, where it is consumed (hipcc by itself copies a hundred of them up front and spills)
+__device__ __forceinline__ float from_acc(float a) {
+    float v;
+    asm("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+    return v;
+}
+
+// ---- the streaming kernel: 256 x 256 tiles, 16-bit results, a workgroup per CU that walks tiles without a pause ----------------------
+// The ring kernel's steps with 4 x 4 matrix tiles per wave, for k a multiple of 128 from 512 on, n a multiple of 8, rows of c on 16 bytes.  There a tile of 16 steps spent 17000 of
+// its 38000 cycles outside its products (start and addresses 5000, first latency 3600, epilogue 8000).  Here the last four steps of a tile
+// already request the first four of the next one; the next tile's scales and bias are loaded in front of the epilogue and written to LDS
+// behind it; and the epilogue needs no LDS: v_permlane32_swap joins the 4 + 4 columns of two lanes into 16 bytes of a row, stored
+// straight from registers.  The wait for those loads (younger than the four steps' requests, same counter) also covers the requests, so
+// steps 0 .. 2 of a tile wait for nothing and its predecessor's stores retire behind them.
+template <typename T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void fp8_gemm_stream_kernel(GemmParams p, int mt, int nt) {
+    static_assert(sizeof(T) == 2, "16-bit results");
+    constexpr int NI = 4, NJ = 4, BN = 256, BM = 256, ROWS = 512, SLOT = ROWS * 64, RING = 4 * SLOT, NQ = 8;
+    __shared__ __attribute__((aligned(16))) char smem[RING + ROWS * G8_SPITCH + 2 * BN * 4];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wn = w & 1, wm = w >> 1;
+    const int ml = lane & 31, hh = lane >> 5;
+    const int nkb = (int)(p.k / QB), nst = 2 * nkb;
+
+    // workgroup -> its tiles: the ring kernel's order, cut into a run per workgroup of an XCD: tile number v, v + grid, ...
+    const int tiles = mt * nt, q8 = tiles >> 3, r8 = tiles & 7;
+    auto place = [&](int v, long& m0, long& n0) {
+        const int xcd = v & 7;
+        const int tile = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (v >> 3);
+        const int grp = tile / (4 * nt), rem = tile - grp * 4 * nt, gm = min(4, mt - grp * 4);
+        m0 = (long)(grp * 4 + rem % gm) * BM, n0 = (long)(rem / gm) * BN;
+    };
+    long m0, n0;
+    place(blockIdx.x, m0, n0);
+
+    unsigned goff[NQ];
+    const uint8_t *rqb, *rqa;
+    auto aim = [&](long tm, long tn) {   // the request stream to the first step of a tile
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            const bool isb = q < NI;
+            const int r = (isb ? (w * NI + q) : (w * NJ + q - NI)) * 16 + (lane >> 2);
+            const int last = (int)min((isb ? p.n - tn : p.m - tm) - 1, 255L);
+            goff[q] = (unsigned)min(r, last) * (unsigned)(isb ? p.ldb : p.lda) + (((lane & 3) ^ ((r >> 2) & 3)) * 16);
+        }
+        rqb = p.b + tn * p.ldb;
+        rqa = p.a + tm * p.lda;
+    };
+    const int lds0 = (int)(size_t)(__attribute__((address_space(3))) char*)smem;
+    auto request = [&](int slot, int q) {
+        const int at = lds0 + slot * SLOT + (q < NI ? (w * NI + q) * 1024 : BN * 64 + (w * NJ + q - NI) * 1024);
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(goff[q]), "s"(q < NI ? rqb : rqa), "s"(at) : "memory");
+    };
+
+    const int swz = (ml >> 2) & 3;
+    const int boff = (wn * 128 + ml) * 64, aoff = BN * 64 + (wm * 128 + ml) * 64;
+    const int c0 = (hh ^ swz) * 16, c1 = ((2 + hh) ^ swz) * 16;
+    struct Frag { i32x8 b[NI], a[NJ]; };
+    auto join = [](u32x4 x, u32x4 y) { return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]}; };
+    auto read_one = [&](Frag& f, const char* slot, int q) {
+        if (q < NI) f.b[q] = join(*(const u32x4*)(slot + boff + q * 2048 + c0), *(const u32x4*)(slot + boff + q * 2048 + c1));
+        else f.a[q - NI] = join(*(const u32x4*)(slot + aoff + (q - NI) * 2048 + c0), *(const u32x4*)(slot + aoff + (q - NI) * 2048 + c1));
+    };
+    unsigned sb[NI], sa[NJ], sbn[NI], san[NJ];
+    char* const slds = smem + RING;
+    float* const bias = (float*)(slds + ROWS * G8_SPITCH);   // of this tile and of the next one, by turns
+    int turn = 0;
+    auto read_scales = [&](int kb) {
+        const char* const at = slds + (kb & (G8_CHUNK - 1));
+#pragma unroll
+        for (int i = 0; i < NI; ++i) sbn[i] = *(const uint8_t*)(at + (wn * 128 + i * 32 + ml) * G8_SPITCH);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) san[j] = *(const uint8_t*)(at + (BN + wm * 128 + j * 32 + ml) * G8_SPITCH);
+    };
+    // scales of blocks kb0 .. kb0 + 31: a thread has one row of b and one of a
+    struct Scales { unsigned v[2][G8_CHUNK / 4]; float bias; };
+    auto load_scales = [&](Scales& t, long tm, long tn, int kb0) {
+        const int have = min(nkb - kb0, G8_CHUNK);
+        const long rb = min(tn + tid, p.n - 1), ra = min(tm + tid, p.m - 1);
+        const uint8_t* const src[2] = {p.sb + (p.b_tile ? rb / QB : rb) * p.ldsb + kb0, p.sa + (p.a_tile ? ra / QB : ra) * p.ldsa + kb0};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < G8_CHUNK / 4; ++j) {
+                t.v[i][j] = 0;
+                if (4 * j + 4 <= have) {
+                    __builtin_memcpy(&t.v[i][j], src[i] + 4 * j, 4);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (4 * j + e < have) t.v[i][j] |= (unsigned)src[i][4 * j + e] << (8 * e);
+                }
+            }
+        t.bias = bias_at(p, tn + tid);
+    };
+    auto write_scales = [&](const Scales& t, int turn) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < G8_CHUNK / 4; ++j) *(unsigned*)(slds + (tid + 256 * i) * G8_SPITCH + 4 * j) = t.v[i][j];
+        bias[turn * BN + tid] = t.bias;
+    };
+
+    f32x16 acc[NI][NJ];
+    int s0 = 0;   // steps of the tiles before this one: the ring goes on
+    // as in the ring kernel; FIRST: the products start from 0, and nothing is waited for in steps 0 .. 2
+    auto step = [&](int s, Frag& FH, Frag& FN, auto odd, auto first, auto wait) {
+        constexpr bool ODD = decltype(odd)::value, FIRST = decltype(first)::value;
+        constexpr int WAIT = decltype(wait)::value;
+        if constexpr (WAIT >= 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(WAIT < 0 ? 0 : WAIT) : "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!ODD) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) sb[i] = sbn[i];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sa[j] = san[j];
+        }
+        const char* const next = smem + ((s0 + s + 1) & 3) * SLOT;
+        const int slot = (s0 + s) & 3;
+#pragma unroll
+        for (int x = 0; x < NI * NJ; ++x) {
+            const int i = x / NJ, j = x % NJ;
+            __builtin_amdgcn_sched_barrier(0);
+            acc[i][j] = mfma64<T>(FH.b[i], FH.a[j], FIRST ? f32x16{} : acc[i][j], sb[i], sa[j]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (x < NQ) read_one(FN, next, x);
+            if (ODD && x == NQ) read_scales((s + 1) >> 1);
+            if (x >= G8_REQ0 && x < G8_REQ0 + NQ) request(slot, x - G8_REQ0);
+        }
+        rqb += 64, rqa += 64;
+    };
+    constexpr std::integral_constant<bool, false> no{};
+    constexpr std::integral_constant<bool, true> yes{};
+    constexpr std::integral_constant<int, 2 * NQ> two{};
+    constexpr std::integral_constant<int, -1> none{};
+
+    Frag f0, f1;
+    aim(m0, n0);
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+        asm volatile("s_nop 4" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) request(st, q);
+        rqb += 64, rqa += 64;
+    }
+    {
+        Scales t;
+        load_scales(t, m0, n0, 0);
+        write_scales(t, 0);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) read_one(f0, smem, q);
+    read_scales(0);
+
+    for (int v = blockIdx.x;;) {
+        const int vn = v + (int)gridDim.x;
+        const bool more = vn < tiles;   // (the same for the whole workgroup)
+        long mn = m0, nn = n0;
+        // (a tile of 8 steps goes over to the next tile's requests behind step 3)
+        step(0, f0, f1, no, yes, none);
+        step(1, f1, f0, yes, no, none);
+        step(2, f0, f1, no, no, none);
+        step(3, f1, f0, yes, no, two);
+#pragma clang loop unroll(disable)
+        for (int s = 4; s < nst; s += 2) {
+            if (s == nst - 4) {   // from here on the next tile's steps (behind the last tile: its own first ones again, which nothing reads)
+                if (more) place(vn, mn, nn);
+                aim(mn, nn);
+                asm volatile("s_nop 4" ::: "memory");
+            }
+            if ((s & (2 * G8_CHUNK - 1)) == 0) {   // the next 32 blocks' scales; nobody reads the last ones' any more
+                Scales t;
+                load_scales(t, m0, n0, s >> 1);
+                write_scales(t, turn);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                read_scales(s >> 1);
+            }
+            step(s, f0, f1, no, no, two);
+            step(s + 1, f1, f0, yes, no, two);   // (the last one: f0 = the next tile's first fragments)
+        }
+
+        // ---- epilogue, with the next tile's scales on their way (the accumulators are read by asm, for which hipcc pads nothing: a
+        // matrix instruction's result may be read 18 wait states behind it)
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        Scales t;
+        load_scales(t, mn, nn, 0);
+        // (16 columns are wholly inside or outside: n is a multiple of 8)
+        T* const out0 = (T*)p.c + (m0 + wm * 128 + ml) * p.ldc + n0 + wn * 128 + 8 * hh;
+        const int rows = (int)min(p.m - (m0 + wm * 128 + ml), 128L), cols = (int)min(p.n - (n0 + wn * 128 + 8 * hh), 128L);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            f32x4 b4[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) b4[g] = *(const f32x4*)(bias + turn * BN + wn * 128 + i * 32 + 8 * g + 4 * hh);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {   // columns 16 h .. 16 h + 15 of the matrix tile: lanes below 32 get the first 8, the others the last
+                    typedef T t2 __attribute__((ext_vector_type(2)));
+                    unsigned d[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int g = 2 * h + (e >> 1), k = 4 * g + 2 * (e & 1);
+                        d[e] = __builtin_bit_cast(unsigned, t2{(T)(from_acc(acc[i][j][k]) + b4[g][2 * (e & 1)]), (T)(from_acc(acc[i][j][k + 1]) + b4[g][2 * (e & 1) + 1])});
+                    }
+                    const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+                    const u32x4 q = {(unsigned)x[0], (unsigned)y[0], (unsigned)x[1], (unsigned)y[1]};
+                    if (j * 32 < rows && i * 32 + h * 16 < cols) *(u32x4*)(out0 + (long)j * 32 * p.ldc + i * 32 + h * 16) = q;
+                }
+        }
+        turn ^= 1;
+        write_scales(t, turn);   // (nobody reads the last scales any more; the bias has its own place)
+        // (its wait: everything older than these loads has landed, the next tile's four steps among it)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (!more) break;
+        read_scales(0);
+        s0 += nst, v = vn, m0 = mn, n0 = nn;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no LDS-DMA is under way when the workgroup gives its LDS back)
 }
 
 // ---- few rows of a: 16 MT x 16 of c per workgroup of 8 waves, which share the blocks of k --------------------------------------

@@ -180,6 +180,44 @@ def test_matmul_large_and_repeatable(cuda_device):
         assert torch.equal(c, fp8.matmul(*dev, out_dtype=torch.float32))
 
 
+@pytest.mark.parametrize('m,n,k,bias', [(4097, 4100, 640, True), (8192, 2048, 512, False), (4096, 4096, 1152, True), (3900, 5120, 4224, False),
+                                        (4352, 4352, 4352, True), (7000, 2300, 1111, True), (66000, 260, 768, True)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_matmul_many_tiles(cuda_device, m, n, k, bias, dtype):
+    """The kernels of large products: several tiles per workgroup, ragged edges, scales of more than 32 blocks (the oracle's products in
+    64 bits on the GPU)."""
+    g = torch.Generator(device='cuda').manual_seed(m + n + k)
+    a = torch.randint(0, 256, (m, k), generator=g, device=cuda_device, dtype=torch.uint8)
+    b = torch.randint(0, 256, (n, k), generator=g, device=cuda_device, dtype=torch.uint8)
+    a, b = (torch.where(t & 0x7f == 0x7f, t - 1, t) for t in (a, b))
+    kb = -(-k // 128)
+    sa = torch.randint(117, 126, (m, kb), generator=g, device=cuda_device, dtype=torch.uint8)
+    sb = torch.randint(117, 126, ((n + 127) // 128 if m % 2 else n, kb), generator=g, device=cuda_device, dtype=torch.uint8)
+    bv = torch.randn(n, generator=g, device=cuda_device) * 100 if bias else None
+    wide = [torch.zeros((t.shape[0], k + -k % 16), dtype=torch.uint8, device=cuda_device) for t in (a, b)]
+    for t, v in zip(wide, (a, b)):
+        t[:, :k] = v
+    wa, wb = (t[:, :k].view(F8) for t in wide)
+    c = fp8.matmul(wa, sa.view(E8), wb, sb.view(E8), bias=bv, out_dtype=dtype)
+
+    def values(x, s):
+        v = torch.pow(2.0, (s.long() - 127).double()).repeat_interleave(128, 1)[:, :k]
+        v = v.repeat_interleave(128, 0)[:x.shape[0]] if s.shape[0] != x.shape[0] else v
+        return x.view(F8).float().double() * v
+
+    av, bw = values(a, sa), values(b, sb)
+    want, mag = av @ bw.t(), av.abs() @ bw.abs().t()
+    if bias:
+        want += bv.double()
+    err = (c.double() - want).abs()
+    fine = torch.isfinite(c) if dtype == torch.float16 else torch.ones_like(c, dtype=torch.bool)
+    assert bool((fine | (want.abs() > 65000)).all())
+    tol = (2 * U * k + 2.0 ** -10) * mag + half(dtype) * 1.01 * want.abs() + 1e-6
+    assert bool((err <= tol)[fine].all())
+    assert float(err[fine].norm()) <= (3.5e-4 + half(dtype)) * float(want[fine].norm())
+    assert torch.equal(c, fp8.matmul(wa, sa.view(E8), wb, sb.view(E8), bias=bv, out_dtype=dtype))
+
+
 def test_matmul_views_pads_and_out(cuda_device):
     """Operands inside wider matrices whose other bytes are NaN codes, unaligned first columns, an output with a row stride."""
     m, n, k = 150, 140, 300
