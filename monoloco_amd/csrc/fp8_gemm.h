@@ -643,27 +643,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void f
         // (16 columns are wholly inside or outside: n is a multiple of 8)
         T* const out0 = (T*)p.c + (m0 + wm * 128 + ml) * p.ldc + n0 + wn * 128 + 8 * hh;
         const int rows = (int)min(p.m - (m0 + wm * 128 + ml), 128L), cols = (int)min(p.n - (n0 + wn * 128 + 8 * hh), 128L);
+        auto columns = [&](auto edge) {   // EDGE: a branch around every store
+            constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            f32x4 b4[4];
+            for (int i = 0; i < NI; ++i) {
+                f32x4 b4[4];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) b4[g] = *(const f32x4*)(bias + turn * BN + wn * 128 + i * 32 + 8 * g + 4 * hh);
+                for (int g = 0; g < 4; ++g) b4[g] = *(const f32x4*)(bias + turn * BN + wn * 128 + i * 32 + 8 * g + 4 * hh);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+                for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {   // columns 16 h .. 16 h + 15 of the matrix tile: lanes below 32 get the first 8, the others the last
-                    typedef T t2 __attribute__((ext_vector_type(2)));
-                    unsigned d[4];
+                    for (int h = 0; h < 2; ++h) {   // columns 16 h .. 16 h + 15 of the matrix tile: lanes below 32 get the first 8, the others the last
+                        typedef T t2 __attribute__((ext_vector_type(2)));
+                        unsigned d[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int g = 2 * h + (e >> 1), k = 4 * g + 2 * (e & 1);
-                        d[e] = __builtin_bit_cast(unsigned, t2{(T)(from_acc(acc[i][j][k]) + b4[g][2 * (e & 1)]), (T)(from_acc(acc[i][j][k + 1]) + b4[g][2 * (e & 1) + 1])});
+                        for (int e = 0; e < 4; ++e) {
+                            const int g = 2 * h + (e >> 1), k = 4 * g + 2 * (e & 1);
+                            d[e] = __builtin_bit_cast(unsigned, t2{(T)(from_acc(acc[i][j][k]) + b4[g][2 * (e & 1)]), (T)(from_acc(acc[i][j][k + 1]) + b4[g][2 * (e & 1) + 1])});
+                        }
+                        const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+                        const u32x4 q = {(unsigned)x[0], (unsigned)y[0], (unsigned)x[1], (unsigned)y[1]};
+                        if (!EDGE || (j * 32 < rows && i * 32 + h * 16 < cols)) *(u32x4*)(out0 + (long)j * 32 * p.ldc + i * 32 + h * 16) = q;
                     }
-                    const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
-                    const u32x4 q = {(unsigned)x[0], (unsigned)y[0], (unsigned)x[1], (unsigned)y[1]};
-                    if (j * 32 < rows && i * 32 + h * 16 < cols) *(u32x4*)(out0 + (long)j * 32 * p.ldc + i * 32 + h * 16) = q;
-                }
-        }
+            }
+        };
+        if (m0 + BM <= p.m && n0 + BN <= p.n) columns(no);
+        else columns(yes);
         turn ^= 1;
         write_scales(t, turn);   // (nobody reads the last scales any more; the bias has its own place)
         // (its wait: everything older than these loads has landed, the next tile's four steps among it)
