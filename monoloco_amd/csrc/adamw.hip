@@ -180,7 +180,7 @@ extern "C" int ml_adamw_step(int n_tensors, const int64_t* numel, void* const* p
     if (step < 1) return ops_fail(ML_ERR_ARG, "ml_adamw_step: steps are counted from 1, got %lld", (long long)step);
     if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0)) return ops_fail(ML_ERR_ARG, "ml_adamw_step: betas are in [0, 1), eps is not negative");
     for (int i = 0; i < n_tensors; ++i) {
-        if (numel[i] < 0 || numel[i] > (1LL << 38)) return ops_fail(ML_ERR_SHAPE, "ml_adamw_step: tensor %d has %lld elements", i, (long long)numel[i]);
+        if (numel[i] < 0 || numel[i] > (1LL << 35)) return ops_fail(ML_ERR_SHAPE, "ml_adamw_step: tensor %d has %lld elements", i, (long long)numel[i]);
         if (numel[i] && (!params[i] || !grads[i] || !exp_avgs[i] || !exp_avg_sqs[i] || (scales && !scales[i]))) return ops_fail(ML_ERR_ARG, "ml_adamw_step: tensor %d has a null pointer", i);
     }
     const hipStream_t s = (hipStream_t)stream;
@@ -197,7 +197,7 @@ extern "C" int ml_adamw_step(int n_tensors, const int64_t* numel, void* const* p
         for (; i < n_tensors && k < MAX_TENSORS; ++i) {
             if (numel[i] == 0) continue;
             const int64_t wgs = (numel[i] + WG_ELEMS - 1) / WG_ELEMS;
-            if (k > 0 && grid + wgs > 0x7fffffffLL) break;   // (one tensor alone always fits: at most 2^26 workgroups)
+            if (k > 0 && grid + wgs > 0xffffffLL) break;   // (a launch has fewer than 2^32 threads; one tensor alone always fits: 2^23 workgroups)
             t.p[k] = params[i], t.g[k] = grads[i], t.m[k] = exp_avgs[i], t.v[k] = exp_avg_sqs[i], t.s[k] = scales ? scales[i] : nullptr;
             t.numel[k] = numel[i], t.first[k] = grid;
             t.key[k] = host_mix32(seed + 0x9e3779b9U * host_mix32((uint32_t)step + 0x85ebca6bU * (uint32_t)(i + 1)));

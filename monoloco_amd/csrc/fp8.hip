@@ -9,8 +9,8 @@ using namespace mlk;
 
 namespace {
 
-constexpr long MAX_GRID = 0x7fffffffL;
-constexpr long G8_FROM256 = 256, G8_FROM128 = 256;
+// a launch has fewer than 2^32 threads
+bool fits(long workgroups, int threads) { return workgroups <= 0xffffffffL / threads; }
 
 int elem_size(int dtype) { return dtype == ML_F32 ? 4 : dtype == ML_BF16 || dtype == ML_F16 ? 2 : 0; }
 
@@ -47,22 +47,41 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
     else rms_norm_back_kernel<T, 16, 0><<<g, 1024, 0, s>>>(p);
 }
 
-// Which product kernel: the ring wants rows that start on 16 bytes and offsets inside a tile below 2^32; its tile is the largest that
-// still gives every CU work.
+// Which product kernel (us measured on both sides of each border, bf16 results unless said):
+//   m <= 32 rows (fp32 results: 64): the waves of a workgroup share k.  4096 x 4096, m = 32: 10.5 against 12.9 with 64 x 64 tiles; m = 64:
+//     16.4 against 13.1, fp32 18.1 against 24.6.
+//   The ring wants rows that start on 16 bytes and offsets inside a tile below 2^32; everything else takes the plain 64 x 64 kernel.
+//   64 x 64 tiles while they fit the CUs once (or, k <= 2048, twice): 512 x 1024 x 1024 6.1 against 7.9 with 128 x 128; 2048 x 1024 x 1024
+//     7.7 against 8.4; 384 x 4096 x 4096 (384 tiles) 22.4 against 18.5.  fp32: while the 128 x 128 tiles are fewer than the CUs.
+//   256 x 256 tiles (16-bit results) once they are more than the CUs, or k >= 2048 and 160 of them: 16384 x 1024 x 1024 (256 tiles) 26.9
+//     against 24.6 with 128 x 128, 32768 x 1024 x 1024 44.7 against 48.9; 2048 x 4096 x 4096 (128) 47.1 against 40.9, 4096^3 (256) 59.7
+//     against 77.9; below k = 1024 a tile's start and end outweigh its steps.
 template <typename T>
-void launch_gemm(const GemmParams& p, unsigned grid64, hipStream_t s) {
+void launch_gemm(const GemmParams& p, hipStream_t s) {
+    constexpr bool HALF = sizeof(T) == 2;
     const bool ring = p.fast_a && p.fast_b && p.lda < (1L << 23) && p.ldb < (1L << 23);
-    const long t256 = ((p.m + 255) / 256) * ((p.n + 255) / 256), t128 = ((p.m + 127) / 128) * ((p.n + 127) / 128);
+    auto across = [&](long t) { return (p.m + t - 1) / t * ((p.n + t - 1) / t); };
+    const long t256 = across(256), t128 = across(128), t64 = across(64);
+    auto tiles = [](long size, int t) { return (int)((size + t - 1) / t); };
     const unsigned g16 = (unsigned)((p.n + 15) / 16);
-    if (p.m <= 16) fp8_gemm_rows_kernel<T, 1, 4><<<g16, 512, 0, s>>>(p);
-    else if (p.m <= 32) fp8_gemm_rows_kernel<T, 2, 2><<<g16, 512, 0, s>>>(p);
-    else if (p.m <= 64) fp8_gemm_rows_kernel<T, 4, 2><<<g16, 512, 0, s>>>(p);
-    else if (ring && sizeof(T) == 2 && t256 >= G8_FROM256 && p.k % QB == 0 && p.k >= 512 && p.n % 8 == 0 && p.vec_c) {
-        if constexpr (sizeof(T) == 2) fp8_gemm_stream_kernel<T><<<(unsigned)(t256 < 256 ? t256 : 256), 256, 0, s>>>(p, (int)((p.m + 255) / 256), (int)((p.n + 255) / 256));
-    } else if (ring && sizeof(T) == 2 && t256 >= G8_FROM256) fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, (int)((p.m + 255) / 256), (int)((p.n + 255) / 256));
-    else if (ring && t128 >= G8_FROM128) fp8_gemm_ring_kernel<T, 2, 2><<<(unsigned)t128, 256, 0, s>>>(p, (int)((p.m + 127) / 128), (int)((p.n + 127) / 128));
-    else if (ring) fp8_gemm_ring_kernel<T, 1, 1><<<grid64, 256, 0, s>>>(p, (int)((p.m + 63) / 64), (int)((p.n + 63) / 64));
-    else fp8_gemm64_kernel<T><<<grid64, 256, 0, s>>>(p);
+    if (p.m <= 16) {
+        fp8_gemm_rows_kernel<T, 1, 4><<<g16, 512, 0, s>>>(p);
+    } else if (p.m <= 32) {
+        fp8_gemm_rows_kernel<T, 2, 2><<<g16, 512, 0, s>>>(p);
+    } else if (!HALF && p.m <= 64) {
+        if constexpr (!HALF) fp8_gemm_rows_kernel<T, 4, 2><<<g16, 512, 0, s>>>(p);
+    } else if (!ring) {
+        fp8_gemm64_kernel<T><<<(unsigned)t64, 256, 0, s>>>(p);
+    } else if (HALF && p.k >= 1024 && (t256 > 256 || (t256 >= 160 && p.k >= 2048))) {
+        if constexpr (HALF) {
+            if (p.k % QB == 0 && p.n % 8 == 0 && p.vec_c) fp8_gemm_stream_kernel<T><<<(unsigned)(t256 < 256 ? t256 : 256), 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
+            else fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
+        }
+    } else if (HALF ? t64 <= (p.k <= 2048 ? 512 : 256) : t128 < 256) {
+        fp8_gemm_ring_kernel<T, 1, 1><<<(unsigned)t64, 256, 0, s>>>(p, tiles(p.m, 64), tiles(p.n, 64));
+    } else {
+        fp8_gemm_ring_kernel<T, 2, 2><<<(unsigned)t128, 256, 0, s>>>(p, tiles(p.m, 128), tiles(p.n, 128));
+    }
 }
 
 // workgroups of the backward pass = rows of its partial sums: enough to fill 256 CUs with 16 waves, few enough that writing and
@@ -81,7 +100,7 @@ int column_sums(const void* x, int dtype, int64_t m, int64_t n, int64_t ldx, flo
     QuantParams p{};
     p.x = x, p.m = m, p.n = n, p.ldx = ldx, p.colsum = out, p.vec = rows_aligned(x, ldx, es, 16);
     const long grid = ((n + QB - 1) / QB) * ((m + QB - 1) / QB);
-    if (grid > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "column sums: %lld x %lld is too large", (long long)m, (long long)n);
+    if (!fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "column sums: %lld x %lld is too large", (long long)m, (long long)n);
     with_type(dtype, [&](auto t) { quantize_tile_kernel<decltype(t)><<<(unsigned)grid, 256, 0, s>>>(p); });
     return ops_launched("column sums");
 }
@@ -111,7 +130,7 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
     const hipStream_t s = (hipStream_t)stream;
     const bool rows = !qt_dev && !tile && !colsum_dev;
     const long grid = rows ? (m * nb + 15) / 16 : mb * nb;
-    if (grid > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_fp8_quantize: %lld x %lld is too large", (long long)m, (long long)n);
+    if (!fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_quantize: %lld x %lld is too large", (long long)m, (long long)n);
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (rows) quantize_rows_kernel<T><<<(unsigned)grid, 256, 0, s>>>(p);
@@ -130,12 +149,12 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
     const long kb = (k + QB - 1) / QB;
     if (lda < k || ldb < k || ldc < n || ldsa < kb || ldsb < kb) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: a row stride is shorter than its row");
     const long grid = ((m + 63) / 64) * ((n + 63) / 64);
-    if (m > (1LL << 40) || n > (1LL << 40) || grid > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
+    if (m > (1LL << 40) || n > (1LL << 33) || !fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
     GemmParams p{a_dev, b_dev, a_scale_dev, b_scale_dev, (long)lda, (long)ldb, (long)ldsa, (long)ldsb, a_tile != 0, b_tile != 0, bias_dev, bias_dtype, c_dev,
                  (long)m, (long)n, (long)k, (long)ldc, 0, 0, 0};
     p.fast_a = rows_aligned(a_dev, lda, 1, 16), p.fast_b = rows_aligned(b_dev, ldb, 1, 16), p.vec_c = rows_aligned(c_dev, ldc, es, 16);
     const hipStream_t s = (hipStream_t)stream;
-    with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, (unsigned)grid, s); });
+    with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, s); });
     return ops_launched("ml_fp8_matmul");
 }
 
@@ -218,7 +237,7 @@ int ml_rms_norm(const void* x_dev, int64_t ldx, const void* residual_dev, int64_
     const long nb = (n + QB - 1) / QB;
     if (ldx < n || (residual_dev && ldr < n) || (h_dev && ldh < n) || (y_dev && ldy < n) || (q_dev && (ldq < n || lds < nb)))
         return ops_fail(ML_ERR_ARG, "ml_rms_norm: a row stride is shorter than its row");
-    if (m > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm: %lld rows are too many", (long long)m);
+    if (!(n <= 2048 ? fits((m + 3) / 4, 256) : fits(m, n <= 8192 ? 256 : 1024))) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm: %lld rows of %lld are too many", (long long)m, (long long)n);
     NormParams p{};
     p.x = x_dev, p.residual = residual_dev, p.w = w_dev, p.w_f32 = w_dtype == ML_F32;
     p.m = m, p.n = n, p.ldx = ldx, p.ldr = ldr, p.ldy = q_dev ? ldq : ldy, p.ldh = ldh, p.eps = eps;
@@ -244,6 +263,7 @@ int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int
     if (n == 0) return ML_OK;
     if (!dw_dev || (m > 0 && (!dy_dev || !h_dev || !w_dev || !dx_dev || !work_dev))) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: null pointer");
     if (m > 0 && (ldy < n || ldh < n || (dh_dev && ldd < n) || ldx < n)) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: a row stride is shorter than its row");
+    if (!fits((n + 31) / 32, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm_backward: %lld columns are too many", (long long)n);
     const hipStream_t s = (hipStream_t)stream;
     const long groups = m ? norm_groups(m, n) : 0;
     if (m > 0) {
@@ -264,7 +284,7 @@ int ml_sum_rows(const float* part_dev, int64_t rows, int64_t n, void* out_dev, i
     if (!elem_size(dtype) || rows < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_sum_rows: bad type %d or size", dtype);
     if (n == 0) return ML_OK;
     if (!out_dev || (rows > 0 && !part_dev)) return ops_fail(ML_ERR_ARG, "ml_sum_rows: null pointer");
-    if ((n + 31) / 32 > MAX_GRID) return ops_fail(ML_ERR_SHAPE, "ml_sum_rows: %lld columns are too many", (long long)n);
+    if (!fits((n + 31) / 32, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_sum_rows: %lld columns are too many", (long long)n);
     with_type(dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + 31) / 32), 1024, 0, (hipStream_t)stream>>>(part_dev, rows, n, (decltype(t)*)out_dev); });
     return ops_launched("ml_sum_rows");
 }

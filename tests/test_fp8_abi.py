@@ -26,7 +26,7 @@ def test_quantize_refusals(hip_lib):
     for ldx, ldq, lds, ldqt, ldst in ((129, 130, 2, 16, 1), (130, 129, 2, 16, 1), (130, 130, 1, 16, 1), (130, 130, 2, 3, 1), (130, 130, 2, 16, 0)):
         _refused(hip_lib, 1, 'row stride', q, P, 0, 4, 130, ldx, 0, P, ldq, P, lds, P, ldqt, P, ldst, None, None)
     _refused(hip_lib, 4, 'too large', q, P, 0, 1 << 41, 4, 4, 0, P, 16, P, 1, None, 0, None, 0, None, None)
-    _refused(hip_lib, 4, 'too large', q, P, 0, 1 << 39, 4, 4, 0, P, 16, P, 1, None, 0, None, 0, None, None)
+    _refused(hip_lib, 4, 'too large', q, P, 0, 1 << 33, 4, 4, 0, P, 16, P, 1, None, 0, None, 0, None, None)
     assert q(None, 0, 0, 4, 4, 0, None, 4, None, 1, None, 0, None, 0, None, None) == 0       # nothing to do
 
 

@@ -180,7 +180,8 @@ def test_matmul_large_and_repeatable(cuda_device):
         assert torch.equal(c, fp8.matmul(*dev, out_dtype=torch.float32))
 
 
-@pytest.mark.parametrize('m,n,k,bias', [(4097, 4100, 640, True), (8192, 2048, 512, False), (4096, 4096, 1152, True), (3900, 5120, 4224, False),
+@pytest.mark.parametrize('m,n,k,bias', [(4097, 4100, 640, True), (8192, 2048, 512, False), (4360, 4104, 1152, True), (3900, 5120, 4224, False), (4104, 4352, 4352, True),
+                                        (4111, 4400, 1024, False), (4111, 4405, 1024, True), (8200, 2056, 2200, False),
                                         (4352, 4352, 4352, True), (7000, 2300, 1111, True), (66000, 260, 768, True)])
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
 def test_matmul_many_tiles(cuda_device, m, n, k, bias, dtype):
