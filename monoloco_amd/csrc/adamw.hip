@@ -11,7 +11,8 @@
 // less than a code's half step, so rounding to nearest would never move it: both are rounded STOCHASTICALLY, up with the probability
 // of the distance, from 16 + 16 random bits per element that depend on the seed, the step, the tensor's place in the call and the
 // element alone (rng.h's generator).  The update itself uses the unrounded m' and r'.  r' > 0 keeps at least the smallest code: a
-// second moment that vanished would let the next step divide by eps.
+// second moment that vanished would let the next step divide by eps.  (eps = 0 and a second moment below fp32's normal range: the divisor
+// is taken as the smallest normal number.)
 #include "block8.h"
 #include "rng.h"
 
@@ -79,12 +80,6 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamTable t, AdamScalars a
     }
 }
 
-// |x| <= 448 times the scale's inverse -> code, rounded up if the fraction plus u / 2^16 reaches 1
-__device__ __forceinline__ unsigned code_stochastic(float x, unsigned u16) {
-    const unsigned sign = __float_as_uint(x) >> 31 << 7, bits = absbits(x);
-    if (bits >= (121u << 23)) return sign | (((bits + (u16 << 4)) >> 20) - (120u << 3));   // 2^-6 and more: 20 bits behind the mantissa's 3
-    return sign | (((unsigned)(__uint_as_float(bits) * 536870912.0f) + (u16 << 4)) >> 20);   // multiples of 2^-9, 20 bits behind
-}
 __device__ __forceinline__ void decode8(u32x2 c, float scale, float (&x)[8]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -100,24 +95,30 @@ __device__ __forceinline__ u32x2 load_codes8(const uint8_t* p, long left, bool v
         if (i < left) c[i >> 2] |= (unsigned)p[i] << (8 * (i & 3));
     return c;
 }
-// 8 new values of a moment -> codes and the block's scale (16 lanes = 128 values)
-__device__ __forceinline__ u32x2 encode8(const float (&x)[8], const unsigned (&u)[8], int shift, bool positive, unsigned& byte) {
+// 8 new values of a moment -> codes and the block's scale (16 lanes = 128 values).  A value of t steps becomes floor(t + u / 2^16): gfx950's
+// stochastic conversion does exactly that with u in the upper half of its random operand, subnormal codes included.  POSITIVE: from one
+// step on (a code of at least 1) unless it is 0.
+template <bool POSITIVE>
+__device__ __forceinline__ u32x2 encode8(const float (&x)[8], const unsigned (&u)[8], unsigned& byte) {
     unsigned a = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) a = max(a, absbits(x[e]));
     byte = scale_byte(max16(a));
-    u32x2 c = {0x7f7f7f7fu, 0x7f7f7f7fu};
-    if (byte != 255) {
-        const float inv = scale_inverse(byte);
-        c[0] = c[1] = 0;
+    if (byte == 255) return u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
+    const float inv = scale_inverse(byte);
+    int c[2] = {0, 0};
+    auto put = [&](int& to, float y, float v, unsigned r, auto sel) {
+        if (POSITIVE && v > 0.0f) y = fmaxf(y, 0.001953125f);
+        to = __builtin_amdgcn_cvt_sr_fp8_f32(y, (int)(POSITIVE ? r & 0xffff0000u : r << 16), to, decltype(sel)::value);
+    };
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            unsigned q = code_stochastic(x[e] * inv, u[e] >> shift & 0xffffu);
-            if (positive && q == 0 && x[e] > 0.0f) q = 1;
-            c[e >> 2] |= q << (8 * (e & 3));
-        }
+    for (int h = 0; h < 2; ++h) {
+        put(c[h], x[4 * h] * inv, x[4 * h], u[4 * h], std::integral_constant<int, 0>{});
+        put(c[h], x[4 * h + 1] * inv, x[4 * h + 1], u[4 * h + 1], std::integral_constant<int, 1>{});
+        put(c[h], x[4 * h + 2] * inv, x[4 * h + 2], u[4 * h + 2], std::integral_constant<int, 2>{});
+        put(c[h], x[4 * h + 3] * inv, x[4 * h + 3], u[4 * h + 3], std::integral_constant<int, 3>{});
     }
-    return c;
+    return u32x2{(unsigned)c[0], (unsigned)c[1]};
 }
 
 template <typename T>
@@ -131,6 +132,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamTable t, AdamScalars a)
     uint8_t* const SM = t.s[k];
     uint8_t* const SR = SM + blocks;
     const unsigned key = t.key[k];
+    const float inv_root = 1.0f / a.root;
     const bool vec = (((uintptr_t)P | (uintptr_t)G) & 15) == 0 && (((uintptr_t)M | (uintptr_t)R) & 7) == 0;
 #pragma unroll
     for (int j = 0; j < WG_ELEMS / 2048; ++j) {
@@ -141,17 +143,21 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamTable t, AdamScalars a)
         load8(G + i, n - i, vec, g);
         decode8(load_codes8(M + i, n - i, vec), scale_value(SM[b]), m);
         decode8(load_codes8(R + i, n - i, vec), scale_value(SR[b]), r);
-        const unsigned bk = mix32(key + (unsigned)b * 0x9e3779b9u);
+        const unsigned bk = mix32(key + (unsigned)b * 0x9e3779b9u) + (unsigned)(i & 127) * 0x85ebca6bu;
         unsigned u[8];
+        // (bound by arithmetic: fused multiply-adds, the hardware's root and reciprocal -- one last place each -- instead of the
+        // correctly rounded ones; 134 M bf16 parameters 355 us before)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            u[e] = mix32(bk + (unsigned)((i + e) & 127) * 0x85ebca6bu);
-            m[e] = m[e] * a.b1 + g[e] * a.c1;
-            r[e] = sqrtf(r[e] * r[e] * a.b2 + g[e] * g[e] * a.c2);
-            p[e] = adam_update(p[e], m[e], r[e], a);
+            u[e] = mix32(bk + (unsigned)e * 0x85ebca6bu);
+            m[e] = fmaf(g[e], a.c1, m[e] * a.b1);
+            r[e] = __builtin_amdgcn_sqrtf(fmaf(g[e] * g[e], a.c2, r[e] * r[e] * a.b2));
+            float den = fmaf(r[e], inv_root, a.eps);
+            den = den < 1.17549435e-38f ? 1.17549435e-38f : den;   // (the reciprocal of a subnormal would be infinite; a NaN stays)
+            p[e] = fmaf(p[e], a.keep, -(a.size * m[e]) * __builtin_amdgcn_rcpf(den));
         }
         unsigned bm, br;
-        const u32x2 cm = encode8(m, u, 0, false, bm), cr = encode8(r, u, 16, true, br);
+        const u32x2 cm = encode8<false>(m, u, bm), cr = encode8<true>(r, u, br);
         if (i < n) {
             store8(P + i, n - i, vec, p);
             store_codes8(M + i, n - i, vec, cm);

@@ -14,6 +14,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/monoloco_hip.h"
 
@@ -53,6 +54,18 @@ __device__ __forceinline__ void vset(Vec8<float>& a, int i, float x) { a.v[i >> 
 __device__ __forceinline__ void vset(Vec8<bf16_t>& a, int i, float x) { a.v[i] = (__bf16)x; }
 __device__ __forceinline__ void vset(Vec8<f16_t>& a, int i, float x) { a.v[i] = (_Float16)x; }
 
+// 8 elements at p as they are: `left` of them exist (<= 0: none), the others are 0; vec: p is 16-byte aligned
+template <typename T>
+__device__ __forceinline__ Vec8<T> load_raw8(const T* p, long left, bool vec) {
+    Vec8<T> v;
+    if (vec && left >= 8) {
+        v = *(const Vec8<T>*)p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vset(v, i, i < left ? (float)p[i] : 0.0f);
+    }
+    return v;
+}
 // 8 elements at p: `left` of them exist (<= 0: none), the others are 0; vec: p is 16-byte aligned
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, long left, bool vec, float (&x)[8]) {
@@ -132,14 +145,17 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, long left, bool vec, u3
     }
 }
 
+// the sum over a wave's 64 lanes, in all of them: four rotations inside rows of 16, then the rows by lane swaps (no LDS)
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-    return x;
-}
-
-template <typename T> __host__ __device__ inline bool aligned(const T* p, long ld, int bytes) {
-    return ((uintptr_t)p % bytes) == 0 && (ld * (long)sizeof(T)) % bytes == 0;
+    auto ror = [](float v, auto ctrl) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false)); };
+    x += ror(x, std::integral_constant<int, 0x128>{});
+    x += ror(x, std::integral_constant<int, 0x124>{});
+    x += ror(x, std::integral_constant<int, 0x122>{});
+    x += ror(x, std::integral_constant<int, 0x121>{});
+    const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+    const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(z[0]) + __uint_as_float(z[1]);
 }
 
 }  // namespace mlk

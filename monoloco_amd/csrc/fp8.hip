@@ -43,7 +43,7 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
     else if (p.n <= 2048) rms_norm_back_kernel<T, 1, 4><<<g, 256, 0, s>>>(p);
     else if (p.n <= 4096) rms_norm_back_kernel<T, 4, 2><<<g, 256, 0, s>>>(p);
     else if (p.n <= 8192) rms_norm_back_kernel<T, 4, 4><<<g, 256, 0, s>>>(p);
-    else if (p.n <= 32768) rms_norm_back_kernel<T, 16, 4><<<g, 1024, 0, s>>>(p);
+    else if (p.n <= 16384) rms_norm_back_kernel<T, 16, 2><<<g, 1024, 0, s>>>(p);   // (four chunks of 16 waves do not fit 128 registers)
     else rms_norm_back_kernel<T, 16, 0><<<g, 1024, 0, s>>>(p);
 }
 

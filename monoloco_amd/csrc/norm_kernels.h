@@ -7,7 +7,8 @@
 // A row stays in registers between its reduction and its output, so everything is read once.  A lane owns chunks of 8 consecutive
 // elements (one 16-byte access of a 2-byte type; 16 neighbouring lanes = one block of 128 of the 8-bit output, whose maximum is
 // four DPP rotations).  WPR = waves per row, NV = chunks per lane: a row of up to 2048 elements is one wave's (no LDS, no barrier;
-// four rows per workgroup), longer ones take 4 or 16 waves; NV = 0 streams rows beyond 32768 elements from memory twice.
+// four rows per workgroup), longer ones take 4 or 16 waves; NV = 0 streams rows beyond 32768
+// elements (backward: 16384) from memory twice.
 #pragma once
 #include "block8.h"
 
@@ -145,25 +146,42 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
     const float inv_n = 1.0f / (float)p.n;
     float* const part = p.part + (long)blockIdx.x * p.n;
     if constexpr (NV > 0) {
-        float dw[NV][8] = {};
-        for (long row = (long)blockIdx.x * TEAMS + team; row < p.m; row += (long)gridDim.x * TEAMS) {
-            float h[NV][8], g[NV][8], ss = 0.0f, gh = 0.0f;
+        // the weight in registers for all rows; the next row's operands are on their way while a row is reduced (65.6 -> 50 us for 32768 x
+        // 1024 in bf16: 4 waves per SIMD alone do not cover the latency), as far as the registers go
+        constexpr bool AHEAD = NV * (int)sizeof(T) <= 4;
+        float dw[NV][8] = {}, wv[NV][8];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) load_weight8<T>(p.w, p.w_f32, lane * 8 + j * STEP, p.n, p.vec, wv[j]);
+        struct Row { Vec8<T> h[NV], g[NV], d[NV]; };
+        auto fetch = [&](Row& r, long row) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const long c = lane * 8 + j * STEP;
-                load8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec, h[j]);
-                load8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec, g[j]);
+                r.h[j] = load_raw8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec);
+                r.g[j] = load_raw8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec);
+                if (p.dh) r.d[j] = load_raw8((const T*)p.dh + row * p.ldd + c, p.n - c, p.vec);
             }
+        };
+        Row now;
+        const long by = (long)gridDim.x * TEAMS;
+        long row = (long)blockIdx.x * TEAMS + team;
+        if (AHEAD && row < p.m) fetch(now, row);
+        for (; row < p.m; row += by) {
+            Row next;
+            if (AHEAD) {
+                if (row + by < p.m) fetch(next, row + by);
+            } else {
+                fetch(now, row);
+            }
+            float ss = 0.0f, gh = 0.0f;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                float wv[8];
-                load_weight8<T>(p.w, p.w_f32, lane * 8 + j * STEP, p.n, p.vec, wv);
+            for (int j = 0; j < NV; ++j)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    ss += h[j][i] * h[j][i];
-                    gh += g[j][i] * wv[i] * h[j][i];
+                    const float h = vget(now.h[j], i);
+                    ss += h * h;
+                    gh += vget(now.g[j], i) * wv[j][i] * h;
                 }
-            }
             ss = row_sum<WPR>(ss, red);
             gh = row_sum<WPR>(gh, red);
             const float rstd = 1.0f / sqrtf(ss * inv_n + p.eps);
@@ -171,17 +189,17 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const long c = lane * 8 + j * STEP;
-                float wv[8], d[8];
-                load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
-                if (p.dh) load8((const T*)p.dh + row * p.ldd + c, p.n - c, p.vec, d);
+                float d[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    dw[j][i] += g[j][i] * (h[j][i] * rstd);
-                    const float v = rstd * (g[j][i] * wv[i] - h[j][i] * k);
-                    d[i] = p.dh ? v + d[i] : v;
+                    const float h = vget(now.h[j], i), g = vget(now.g[j], i);
+                    dw[j][i] += g * (h * rstd);
+                    d[i] = rstd * (g * wv[j][i] - h * k);
+                    if (p.dh) d[i] += vget(now.d[j], i);
                 }
                 if (c < p.n) store8((T*)p.dx + row * p.ldx + c, p.n - c, p.vec, d);
             }
+            if (AHEAD) now = next;
         }
         if (TEAMS > 1) {
             if (team > 0) {
@@ -240,7 +258,8 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
     }
 }
 
-// out[c] = sum over g of part[g * n + c], in a fixed order: 32 columns per workgroup, 32 teams take g = t, t + 32, ...
+// out[c] = sum over g of part[g * n + c], in a fixed order: 32 columns per workgroup, 32 teams take g = t, t + 32, ..., eight loads of
+// each in flight (one after the other they cost 11 us for 1024 x 1024)
 template <typename T>
 __global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restrict__ part, long groups, long n, T* __restrict__ out) {
     __shared__ float s[32][33];
@@ -248,7 +267,12 @@ __global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restri
     const long c = (long)blockIdx.x * 32 + cx;
     float a = 0.0f;
     if (c < n)
-        for (long g = t; g < groups; g += 32) a += part[g * n + c];
+        for (long g = t; g < groups; g += 256) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = g + 32 * u < groups ? part[(g + 32 * u) * n + c] : 0.0f;
+            a += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
     s[t][cx] = a;
     __syncthreads();
     if (t == 0 && c < n) {
