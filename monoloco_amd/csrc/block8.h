@@ -158,4 +158,15 @@ __device__ __forceinline__ float wave_sum(float x) {
     return __uint_as_float(z[0]) + __uint_as_float(z[1]);
 }
 
+// 16 codes to memory: `left` of them exist; vec: p is 16-byte aligned
+__device__ __forceinline__ void store_codes16(uint8_t* p, long left, bool vec, u32x4 c) {
+    if (vec && left >= 16) {
+        *(u32x4*)p = c;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < left) p[i] = (uint8_t)(c[i >> 2] >> (8 * (i & 3)));
+    }
+}
+
 }  // namespace mlk

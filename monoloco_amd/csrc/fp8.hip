@@ -126,7 +126,7 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
     p.x = x_dev, p.m = m, p.n = n, p.ldx = ldx, p.tile = tile != 0;
     p.q = q_dev, p.scale = scale_dev, p.ldq = ldq, p.lds = lds;
     p.qt = qt_dev, p.scale_t = scale_t_dev, p.ldqt = ldqt, p.ldst = ldst, p.colsum = colsum_dev;
-    p.vec = rows_aligned(x_dev, ldx, es, 16), p.vecq = rows_aligned(q_dev, ldq, 1, 8), p.vecqt = rows_aligned(qt_dev, ldqt, 1, 8);
+    p.vec = rows_aligned(x_dev, ldx, es, 16), p.vecq = rows_aligned(q_dev, ldq, 1, 16), p.vecqt = rows_aligned(qt_dev, ldqt, 1, 16);
     const hipStream_t s = (hipStream_t)stream;
     const bool rows = !qt_dev && !tile && !colsum_dev;
     const long grid = rows ? (m * nb + 15) / 16 : mb * nb;

@@ -37,89 +37,111 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantParams p) {
     if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + b] = (uint8_t)byte;
 }
 
-// a 128 x 128 tile per workgroup of 256 threads: thread (tr, tc) = (t / 16, t % 16) holds rows 8 tr .. + 7, columns 8 tc .. + 7
+// a 128 x 128 tile per workgroup of 256 threads: thread (tr, tc) = (t / 16, t % 16) holds rows 8 tr .. + 7, columns 8 tc .. + 7 as they
+// came (fp32 copies of them would cost half the occupancy).  Rows are stored 16 bytes a lane (two lanes trade rows for columns); the
+// transposed tile goes through LDS, its 16-byte pieces exchanged by row / 8 against bank conflicts.
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_tile_kernel(QuantParams p) {
-    constexpr int PITCH = QB + 8;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void quantize_tile_kernel(QuantParams p) {
     __shared__ unsigned cmax[4][QB];
     __shared__ float csum[4][QB];
-    __shared__ __attribute__((aligned(16))) uint8_t tq[QB * PITCH];
+    __shared__ __attribute__((aligned(16))) uint8_t tq[QB * QB];
     const int tc = threadIdx.x & 15, tr = threadIdx.x >> 4, wave = threadIdx.x >> 6;
-    const long nb = (p.n + QB - 1) / QB, mb = (p.m + QB - 1) / QB;
+    const long nb = (p.n + QB - 1) / QB;
     const long bi = blockIdx.x / nb, bj = blockIdx.x - bi * nb;
     const long r0 = bi * QB + tr * 8, c0 = bj * QB + tc * 8;
-    float x[8][8];
+    Vec8<T> x[8];
     unsigned rmax[8], colmax[8] = {};
 #pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = load_raw8((const T*)p.x + (r0 + i) * p.ldx + c0, r0 + i < p.m ? p.n - c0 : 0, p.vec);
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-        load8((const T*)p.x + (r0 + i) * p.ldx + c0, r0 + i < p.m ? p.n - c0 : 0, p.vec, x[i]);
         rmax[i] = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            rmax[i] = max(rmax[i], absbits(x[i][j]));
-            colmax[j] = max(colmax[j], absbits(x[i][j]));
+            const unsigned a = absbits(vget(x[i], j));
+            rmax[i] = max(rmax[i], a);
+            colmax[j] = max(colmax[j], a);
         }
         rmax[i] = max16(rmax[i]);
     }
     // columns (and sums): over the four row groups of a wave, then over the four waves
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        colmax[j] = max(colmax[j], (unsigned)__shfl_xor((int)colmax[j], 16));
-        colmax[j] = max(colmax[j], (unsigned)__shfl_xor((int)colmax[j], 32));
-        if ((threadIdx.x & 48) == 0) cmax[wave][tc * 8 + j] = colmax[j];
+        const auto y = __builtin_amdgcn_permlane16_swap(colmax[j], colmax[j], false, false);
+        const unsigned h = max((unsigned)y[0], (unsigned)y[1]);
+        const auto z = __builtin_amdgcn_permlane32_swap(h, h, false, false);
+        if ((threadIdx.x & 48) == 0) cmax[wave][tc * 8 + j] = max((unsigned)z[0], (unsigned)z[1]);
         if (p.colsum) {
             float s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += x[i][j];
+            for (int i = 0; i < 8; ++i) s += vget(x[i], j);
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
             if ((threadIdx.x & 48) == 0) csum[wave][tc * 8 + j] = s;
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int c = tc * 8 + j;
-        colmax[j] = max(max(cmax[0][c], cmax[1][c]), max(cmax[2][c], cmax[3][c]));
-        if (p.colsum && tr == 0 && c0 + j < p.n) p.colsum[bi * p.n + c0 + j] = (csum[0][c] + csum[1][c]) + (csum[2][c] + csum[3][c]);
-    }
     unsigned tb = 0;
     if (p.tile) {
         unsigned a = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a = max(a, colmax[j]);
+        for (int j = 0; j < 8; ++j) a = max(a, max(max(cmax[0][tc * 8 + j], cmax[1][tc * 8 + j]), max(cmax[2][tc * 8 + j], cmax[3][tc * 8 + j])));
         tb = scale_byte(max16(a));
     }
+    if (p.colsum && threadIdx.x < QB && bj * QB + threadIdx.x < p.n) {
+        const int c = threadIdx.x;
+        p.colsum[bi * p.n + bj * QB + c] = (csum[0][c] + csum[1][c]) + (csum[2][c] + csum[3][c]);
+    }
     if (p.q) {
+        const bool odd = tc & 1;
+        const long cc = c0 - (odd ? 8 : 0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const unsigned byte = p.tile ? tb : scale_byte(rmax[i]);
-            if (r0 + i < p.m && c0 < p.n) store_codes8(p.q + (r0 + i) * p.ldq + c0, p.n - c0, p.vecq, codes8(x[i], byte));
-            if (!p.tile && tc == 0 && r0 + i < p.m) p.scale[(r0 + i) * p.lds + bj] = (uint8_t)byte;
+        for (int i = 0; i < 8; i += 2) {
+            u32x2 own[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const unsigned byte = p.tile ? tb : scale_byte(rmax[i + e]);
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = vget(x[i + e], j);
+                own[e] = codes8(v, byte);
+                if (!p.tile && tc == 0 && r0 + i + e < p.m) p.scale[(r0 + i + e) * p.lds + bj] = (uint8_t)byte;
+            }
+            // even lanes keep row i and get the odd neighbour's 8 columns of it; odd lanes row i + 1
+            u32x4 v;
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const unsigned give = odd ? own[0][d] : own[1][d], keep = odd ? own[1][d] : own[0][d];
+                const unsigned got = (unsigned)__builtin_amdgcn_update_dpp(0, (int)give, 0xb1, 0xf, 0xf, false);   // quad_perm 1 0 3 2
+                v[d] = odd ? got : keep;
+                v[2 + d] = odd ? keep : got;
+            }
+            const long row = r0 + i + (odd ? 1 : 0);
+            if (row < p.m && cc < p.n) store_codes16(p.q + row * p.ldq + cc, p.n - cc, p.vecq, v);
         }
         if (p.tile && threadIdx.x == 0) p.scale[bi * p.lds + bj] = (uint8_t)tb;
     }
     if (p.qt) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const unsigned byte = p.tile ? tb : scale_byte(colmax[j]);
+            const int c = tc * 8 + j;
+            const unsigned byte = p.tile ? tb : scale_byte(max(max(cmax[0][c], cmax[1][c]), max(cmax[2][c], cmax[3][c])));
             float col[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) col[i] = x[i][j];
-            *(u32x2*)(tq + (tc * 8 + j) * PITCH + tr * 8) = codes8(col, byte);
+            for (int i = 0; i < 8; ++i) col[i] = vget(x[i], j);
+            *(u32x2*)(tq + c * QB + (((tr >> 1) ^ (tc & 7)) * 16) + (tr & 1) * 8) = codes8(col, byte);
             if (!p.tile && tr == 0 && c0 + j < p.n) p.scale_t[(c0 + j) * p.ldst + bi] = (uint8_t)byte;
         }
         if (p.tile && threadIdx.x == 0) p.scale_t[bj * p.ldst + bi] = (uint8_t)tb;
         __syncthreads();
-        // row c of the transposed tile: 16 lanes x 8 bytes
+        // row c of the transposed tile: 8 lanes x 16 bytes
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int c = tr + 16 * k;
-            const long rt = bj * QB + c, ct = bi * QB + tc * 8;
-            if (rt < p.n && ct < p.m) store_codes8(p.qt + rt * p.ldqt + ct, p.m - ct, p.vecqt, *(const u32x2*)(tq + c * PITCH + tc * 8));
+        for (int k = 0; k < 4; ++k) {
+            const int c = (threadIdx.x >> 3) + 32 * k, ch = threadIdx.x & 7;
+            const long rt = bj * QB + c, ct = bi * QB + ch * 16;
+            if (rt < p.n && ct < p.m) store_codes16(p.qt + rt * p.ldqt + ct, p.m - ct, p.vecqt, *(const u32x4*)(tq + c * QB + ((ch ^ ((c >> 3) & 7)) * 16)));
         }
     }
-    (void)mb;
 }
 
 }  // namespace mlk
