@@ -38,7 +38,7 @@ struct AdamScalars {
     float b1, c1, b2, c2, size, root, eps, keep;   // c = 1 - b; size = lr / (1 - b1^t); root = sqrt(1 - b2^t); keep = 1 - lr wd
 };
 
-constexpr int WG_ELEMS = 4096;   // elements per workgroup: 256 threads, 2 chunks of 8 each
+constexpr int WG_ELEMS = 4096;   // elements per workgroup: 256 threads, 4 chunks of 4 (8-bit moments: 2 of 8) each
 
 __device__ __forceinline__ float adam_update(float p, float m, float r, const AdamScalars& a) {
     return p * a.keep - a.size * m / (r / a.root + a.eps);
@@ -58,25 +58,48 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamTable t, AdamScalars a
     const T* const G = (const T*)t.g[k];
     float* const M = (float*)t.m[k];
     float* const V = (float*)t.v[k];
-    const bool vec = (((uintptr_t)P | (uintptr_t)G | (uintptr_t)M | (uintptr_t)V) & 15) == 0;
+    // 4 elements a lane: 16 contiguous bytes of every fp32 array (8 of them, two accesses 32 bytes apart, cost 56 instead of 47 us for 8.4 M
+    // parameters); all loads of the four chunks in flight
+    const bool vec = (((uintptr_t)M | (uintptr_t)V) & 15) == 0 && (((uintptr_t)P | (uintptr_t)G) & (4 * sizeof(T) - 1)) == 0;
+    constexpr int CHUNKS = WG_ELEMS / 1024;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 p[CHUNKS], g[CHUNKS];
+    f32x4 m[CHUNKS], v[CHUNKS];
+    auto fetch = [&](auto& x, const auto* from, long i) {
+        if (vec && i + 4 <= n) {
+            x = *(const std::remove_reference_t<decltype(x)>*)(from + i);
+        } else {
 #pragma unroll
-    for (int j = 0; j < WG_ELEMS / 2048; ++j) {
-        const long i = base + j * 2048 + threadIdx.x * 8;
-        if (i >= n) break;
-        float p[8], g[8], m[8], v[8];
-        load8(P + i, n - i, vec, p);
-        load8(G + i, n - i, vec, g);
-        load8(M + i, n - i, vec, m);
-        load8(V + i, n - i, vec, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            m[e] = m[e] * a.b1 + g[e] * a.c1;
-            v[e] = v[e] * a.b2 + g[e] * g[e] * a.c2;
-            p[e] = adam_update(p[e], m[e], sqrtf(v[e]), a);
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n) x[e] = from[i + e];
         }
-        store8(P + i, n - i, vec, p);
-        store8(M + i, n - i, vec, m);
-        store8(V + i, n - i, vec, v);
+    };
+    auto keep = [&](const auto& x, auto* to, long i) {
+        if (vec && i + 4 <= n) {
+            *(std::remove_cv_t<std::remove_reference_t<decltype(x)>>*)(to + i) = x;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n) to[i + e] = x[e];
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+        const long i = base + j * 1024 + threadIdx.x * 4;
+        p[j] = g[j] = t4{}, m[j] = v[j] = f32x4{};
+        fetch(p[j], P, i), fetch(g[j], G, i), fetch(m[j], (const float*)M, i), fetch(v[j], (const float*)V, i);
+    }
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+        const long i = base + j * 1024 + threadIdx.x * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float ge = (float)g[j][e];
+            m[j][e] = m[j][e] * a.b1 + ge * a.c1;
+            v[j][e] = v[j][e] * a.b2 + ge * ge * a.c2;
+            p[j][e] = (T)adam_update((float)p[j][e], m[j][e], sqrtf(v[j][e]), a);
+        }
+        keep(p[j], P, i), keep(m[j], M, i), keep(v[j], V, i);
     }
 }
 
@@ -145,13 +168,13 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamTable t, AdamScalars a)
         decode8(load_codes8(R + i, n - i, vec), scale_value(SR[b]), r);
         const unsigned bk = mix32(key + (unsigned)b * 0x9e3779b9u) + (unsigned)(i & 127) * 0x85ebca6bu;
         unsigned u[8];
-        // (bound by arithmetic: fused multiply-adds, the hardware's root and reciprocal -- one last place each -- instead of the
-        // correctly rounded ones; 134 M bf16 parameters 355 us before)
+        // (the moments in the 32-bit kernel's operations; root and reciprocal are the hardware's, off by one last place: with the correctly
+        // rounded root and two divisions arithmetic was the bound, 355 us for 134 M bf16 parameters)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             u[e] = mix32(bk + (unsigned)e * 0x85ebca6bu);
-            m[e] = fmaf(g[e], a.c1, m[e] * a.b1);
-            r[e] = __builtin_amdgcn_sqrtf(fmaf(g[e] * g[e], a.c2, r[e] * r[e] * a.b2));
+            m[e] = m[e] * a.b1 + g[e] * a.c1;
+            r[e] = __builtin_amdgcn_sqrtf(r[e] * r[e] * a.b2 + g[e] * g[e] * a.c2);
             float den = fmaf(r[e], inv_root, a.eps);
             den = den < 1.17549435e-38f ? 1.17549435e-38f : den;   // (the reciprocal of a subnormal would be infinite; a NaN stays)
             p[e] = fmaf(p[e], a.keep, -(a.size * m[e]) * __builtin_amdgcn_rcpf(den));

@@ -42,6 +42,10 @@ __device__ __forceinline__ float row_sum(float x, float* red) {
     return s;
 }
 
+// 1 / sqrt(ss / n + eps), once per row, in 64 bits: what the row shares should not add to its elements' own roundings (8-bit codes next to a
+// border would follow it)
+__device__ __forceinline__ float row_rstd(float ss, long n, float eps) { return (float)(1.0 / sqrt((double)ss / (double)n + (double)eps)); }
+
 template <typename T>
 __device__ __forceinline__ void load_weight8(const void* w, int w_f32, long c, long n, bool vec, float (&x)[8]) {
     if (w_f32) load8((const float*)w + c, n - c, vec, x);
@@ -96,7 +100,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_kernel(Nor
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss += h[j][i] * h[j][i];
         }
-        const float rstd = 1.0f / sqrtf(row_sum<WPR>(ss, red) / (float)p.n + p.eps);
+        const float rstd = row_rstd(row_sum<WPR>(ss, red), p.n, p.eps);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const long c = lane * 8 + j * STEP;
@@ -111,7 +115,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_kernel(Nor
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss += h[i] * h[i];
         }
-        const float rstd = 1.0f / sqrtf(row_sum<WPR>(ss, red) / (float)p.n + p.eps);
+        const float rstd = row_rstd(row_sum<WPR>(ss, red), p.n, p.eps);
         for (long c = lane * 8; c < end; c += STEP) {
             norm_in<T>(p, row, c, h);
             if (p.h && c < p.n) store8((T*)p.h + row * p.ldh + c, p.n - c, p.vec, h);
@@ -184,7 +188,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
                 }
             ss = row_sum<WPR>(ss, red);
             gh = row_sum<WPR>(gh, red);
-            const float rstd = 1.0f / sqrtf(ss * inv_n + p.eps);
+            const float rstd = row_rstd(ss, p.n, p.eps);
             const float k = rstd * rstd * (gh * inv_n);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -238,7 +242,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
             }
             ss = row_sum<WPR>(ss, red);
             gh = row_sum<WPR>(gh, red);
-            const float rstd = 1.0f / sqrtf(ss * inv_n + p.eps);
+            const float rstd = row_rstd(ss, p.n, p.eps);
             const float k = rstd * rstd * (gh * inv_n);
             for (long c = lane * 8; c < p.n; c += STEP) {
                 float d[8];
