@@ -60,14 +60,13 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamTable t, AdamScalars a
     float* const V = (float*)t.v[k];
     // 4 elements a lane: 16 contiguous bytes of every fp32 array (8 of them, two accesses 32 bytes apart, cost 56 instead of 47 us for 8.4 M
     // parameters); all loads of the four chunks in flight
-    const bool vec = (((uintptr_t)M | (uintptr_t)V) & 15) == 0 && (((uintptr_t)P | (uintptr_t)G) & (4 * sizeof(T) - 1)) == 0;
     constexpr int CHUNKS = WG_ELEMS / 1024;
     typedef T t4 __attribute__((ext_vector_type(4)));
     t4 p[CHUNKS], g[CHUNKS];
     f32x4 m[CHUNKS], v[CHUNKS];
     auto fetch = [&](auto& x, const auto* from, long i) {
-        if (vec && i + 4 <= n) {
-            x = *(const std::remove_reference_t<decltype(x)>*)(from + i);
+        if (i + 4 <= n) {
+            x = load_any<std::remove_reference_t<decltype(x)>>(from + i);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -75,8 +74,8 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamTable t, AdamScalars a
         }
     };
     auto keep = [&](const auto& x, auto* to, long i) {
-        if (vec && i + 4 <= n) {
-            *(std::remove_cv_t<std::remove_reference_t<decltype(x)>>*)(to + i) = x;
+        if (i + 4 <= n) {
+            store_any(to + i, x);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -110,8 +109,8 @@ __device__ __forceinline__ void decode8(u32x2 c, float scale, float (&x)[8]) {
         x[h * 4] = lo[0] * scale, x[h * 4 + 1] = lo[1] * scale, x[h * 4 + 2] = hi[0] * scale, x[h * 4 + 3] = hi[1] * scale;
     }
 }
-__device__ __forceinline__ u32x2 load_codes8(const uint8_t* p, long left, bool vec) {
-    if (vec && left >= 8) return *(const u32x2*)p;
+__device__ __forceinline__ u32x2 load_codes8(const uint8_t* p, long left) {
+    if (left >= 8) return load_any<u32x2>(p);
     u32x2 c = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -156,16 +155,15 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamTable t, AdamScalars a)
     uint8_t* const SR = SM + blocks;
     const unsigned key = t.key[k];
     const float inv_root = 1.0f / a.root;
-    const bool vec = (((uintptr_t)P | (uintptr_t)G) & 15) == 0 && (((uintptr_t)M | (uintptr_t)R) & 7) == 0;
 #pragma unroll
     for (int j = 0; j < WG_ELEMS / 2048; ++j) {
         const long i = base + j * 2048 + threadIdx.x * 8, b = i / QB;
         if (b >= blocks) break;   // (16 lanes together)
         float p[8], g[8], m[8], r[8];
-        load8(P + i, n - i, vec, p);
-        load8(G + i, n - i, vec, g);
-        decode8(load_codes8(M + i, n - i, vec), scale_value(SM[b]), m);
-        decode8(load_codes8(R + i, n - i, vec), scale_value(SR[b]), r);
+        load8(P + i, n - i, p);
+        load8(G + i, n - i, g);
+        decode8(load_codes8(M + i, n - i), scale_value(SM[b]), m);
+        decode8(load_codes8(R + i, n - i), scale_value(SR[b]), r);
         const unsigned bk = mix32(key + (unsigned)b * 0x9e3779b9u) + (unsigned)(i & 127) * 0x85ebca6bu;
         unsigned u[8];
         // (the moments in the 32-bit kernel's operations; root and reciprocal are the hardware's, off by one last place: with the correctly
@@ -182,9 +180,9 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamTable t, AdamScalars a)
         unsigned bm, br;
         const u32x2 cm = encode8<false>(m, u, bm), cr = encode8<true>(r, u, br);
         if (i < n) {
-            store8(P + i, n - i, vec, p);
-            store_codes8(M + i, n - i, vec, cm);
-            store_codes8(R + i, n - i, vec, cr);
+            store8(P + i, n - i, p);
+            store_codes8(M + i, n - i, cm);
+            store_codes8(R + i, n - i, cr);
         }
         if ((threadIdx.x & 15) == 0) SM[b] = (uint8_t)bm, SR[b] = (uint8_t)br;
     }

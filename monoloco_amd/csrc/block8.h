@@ -54,37 +54,40 @@ __device__ __forceinline__ void vset(Vec8<float>& a, int i, float x) { a.v[i >> 
 __device__ __forceinline__ void vset(Vec8<bf16_t>& a, int i, float x) { a.v[i] = (__bf16)x; }
 __device__ __forceinline__ void vset(Vec8<f16_t>& a, int i, float x) { a.v[i] = (_Float16)x; }
 
-// 8 elements at p as they are: `left` of them exist (<= 0: none), the others are 0; vec: p is 16-byte aligned
+// Rows need no alignment: compute kernels run with unaligned access enabled, and hipcc turns a copy of 16 bytes from any address into one
+// 16-byte access.  (Element by element, 32768 rows of 1023 bf16 took 137 us through the norm; so 46, as rows of 1024 do.)
+template <typename V> __device__ __forceinline__ V load_any(const void* p) {
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+template <typename V> __device__ __forceinline__ void store_any(void* p, const V& v) { __builtin_memcpy(p, &v, sizeof(V)); }
+
+// 8 elements at p as they are: `left` of them exist (<= 0: none), the others are 0
 template <typename T>
-__device__ __forceinline__ Vec8<T> load_raw8(const T* p, long left, bool vec) {
+__device__ __forceinline__ Vec8<T> load_raw8(const T* p, long left) {
     Vec8<T> v;
-    if (vec && left >= 8) {
-        v = *(const Vec8<T>*)p;
+    if (left >= 8) {
+        v = load_any<Vec8<T>>(p);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) vset(v, i, i < left ? (float)p[i] : 0.0f);
     }
     return v;
 }
-// 8 elements at p: `left` of them exist (<= 0: none), the others are 0; vec: p is 16-byte aligned
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, long left, bool vec, float (&x)[8]) {
-    if (vec && left >= 8) {
-        const Vec8<T> v = *(const Vec8<T>*)p;
+__device__ __forceinline__ void load8(const T* p, long left, float (&x)[8]) {
+    const Vec8<T> v = load_raw8(p, left);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = vget(v, i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i < left ? (float)p[i] : 0.0f;
-    }
+    for (int i = 0; i < 8; ++i) x[i] = vget(v, i);
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, long left, bool vec, const float (&x)[8]) {
-    if (vec && left >= 8) {
+__device__ __forceinline__ void store8(T* p, long left, const float (&x)[8]) {
+    if (left >= 8) {
         Vec8<T> v;
 #pragma unroll
         for (int i = 0; i < 8; ++i) vset(v, i, x[i]);
-        *(Vec8<T>*)p = v;
+        store_any(p, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -134,10 +137,10 @@ __device__ __forceinline__ u32x2 codes8(const float (&x)[8], unsigned byte) {
     }
     return r;
 }
-// 8 codes to memory: `left` of them exist; vec: p is 8-byte aligned
-__device__ __forceinline__ void store_codes8(uint8_t* p, long left, bool vec, u32x2 c) {
-    if (vec && left >= 8) {
-        *(u32x2*)p = c;
+// 8 codes to memory: `left` of them exist
+__device__ __forceinline__ void store_codes8(uint8_t* p, long left, u32x2 c) {
+    if (left >= 8) {
+        store_any(p, c);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -158,10 +161,10 @@ __device__ __forceinline__ float wave_sum(float x) {
     return __uint_as_float(z[0]) + __uint_as_float(z[1]);
 }
 
-// 16 codes to memory: `left` of them exist; vec: p is 16-byte aligned
-__device__ __forceinline__ void store_codes16(uint8_t* p, long left, bool vec, u32x4 c) {
-    if (vec && left >= 16) {
-        *(u32x4*)p = c;
+// 16 codes to memory: `left` of them exist
+__device__ __forceinline__ void store_codes16(uint8_t* p, long left, u32x4 c) {
+    if (left >= 16) {
+        store_any(p, c);
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i)

@@ -32,6 +32,7 @@ void launch_norm(const NormParams& p, hipStream_t s) {
     else if (p.n <= 2048) rms_norm_kernel<T, OUT8, 1, 4><<<g4, 256, 0, s>>>(p);
     else if (p.n <= 4096) rms_norm_kernel<T, OUT8, 4, 2><<<g1, 256, 0, s>>>(p);
     else if (p.n <= 8192) rms_norm_kernel<T, OUT8, 4, 4><<<g1, 256, 0, s>>>(p);
+    else if (p.n <= 16384) rms_norm_kernel<T, OUT8, 8, 4><<<g1, 512, 0, s>>>(p);
     else if (p.n <= 32768) rms_norm_kernel<T, OUT8, 16, 4><<<g1, 1024, 0, s>>>(p);
     else rms_norm_kernel<T, OUT8, 16, 0><<<g1, 1024, 0, s>>>(p);
 }
@@ -43,7 +44,7 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
     else if (p.n <= 2048) rms_norm_back_kernel<T, 1, 4><<<g, 256, 0, s>>>(p);
     else if (p.n <= 4096) rms_norm_back_kernel<T, 4, 2><<<g, 256, 0, s>>>(p);
     else if (p.n <= 8192) rms_norm_back_kernel<T, 4, 4><<<g, 256, 0, s>>>(p);
-    else if (p.n <= 16384) rms_norm_back_kernel<T, 16, 2><<<g, 1024, 0, s>>>(p);   // (four chunks of 16 waves do not fit 128 registers)
+    else if (p.n <= 16384) rms_norm_back_kernel<T, 8, 4><<<g, 512, 0, s>>>(p);   // (16 waves leave 128 registers each: spills)
     else rms_norm_back_kernel<T, 16, 0><<<g, 1024, 0, s>>>(p);
 }
 
@@ -74,7 +75,7 @@ void launch_gemm(const GemmParams& p, hipStream_t s) {
         fp8_gemm64_kernel<T><<<(unsigned)t64, 256, 0, s>>>(p);
     } else if (HALF && p.k >= 1024 && (t256 > 256 || (t256 >= 160 && p.k >= 2048))) {
         if constexpr (HALF) {
-            if (p.k % QB == 0 && p.n % 8 == 0 && p.vec_c) fp8_gemm_stream_kernel<T><<<(unsigned)(t256 < 256 ? t256 : 256), 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
+            if (p.k % QB == 0 && p.n % 8 == 0) fp8_gemm_stream_kernel<T><<<(unsigned)(t256 < 256 ? t256 : 256), 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
             else fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
         }
     } else if (HALF ? t64 <= (p.k <= 2048 ? 512 : 256) : t128 < 256) {
@@ -98,7 +99,7 @@ int column_sums(const void* x, int dtype, int64_t m, int64_t n, int64_t ldx, flo
     if (!es || (m && n && ldx < n)) return ops_fail(ML_ERR_ARG, "column sums: bad type %d or row stride", dtype);
     if (m == 0 || n == 0) return ML_OK;
     QuantParams p{};
-    p.x = x, p.m = m, p.n = n, p.ldx = ldx, p.colsum = out, p.vec = rows_aligned(x, ldx, es, 16);
+    p.x = x, p.m = m, p.n = n, p.ldx = ldx, p.colsum = out;
     const long grid = ((n + QB - 1) / QB) * ((m + QB - 1) / QB);
     if (!fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "column sums: %lld x %lld is too large", (long long)m, (long long)n);
     with_type(dtype, [&](auto t) { quantize_tile_kernel<decltype(t)><<<(unsigned)grid, 256, 0, s>>>(p); });
@@ -126,7 +127,6 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
     p.x = x_dev, p.m = m, p.n = n, p.ldx = ldx, p.tile = tile != 0;
     p.q = q_dev, p.scale = scale_dev, p.ldq = ldq, p.lds = lds;
     p.qt = qt_dev, p.scale_t = scale_t_dev, p.ldqt = ldqt, p.ldst = ldst, p.colsum = colsum_dev;
-    p.vec = rows_aligned(x_dev, ldx, es, 16), p.vecq = rows_aligned(q_dev, ldq, 1, 16), p.vecqt = rows_aligned(qt_dev, ldqt, 1, 16);
     const hipStream_t s = (hipStream_t)stream;
     const bool rows = !qt_dev && !tile && !colsum_dev;
     const long grid = rows ? (m * nb + 15) / 16 : mb * nb;
@@ -151,8 +151,8 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
     const long grid = ((m + 63) / 64) * ((n + 63) / 64);
     if (m > (1LL << 40) || n > (1LL << 33) || !fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
     GemmParams p{a_dev, b_dev, a_scale_dev, b_scale_dev, (long)lda, (long)ldb, (long)ldsa, (long)ldsb, a_tile != 0, b_tile != 0, bias_dev, bias_dtype, c_dev,
-                 (long)m, (long)n, (long)k, (long)ldc, 0, 0, 0};
-    p.fast_a = rows_aligned(a_dev, lda, 1, 16), p.fast_b = rows_aligned(b_dev, ldb, 1, 16), p.vec_c = rows_aligned(c_dev, ldc, es, 16);
+                 (long)m, (long)n, (long)k, (long)ldc, 0, 0};
+    p.fast_a = rows_aligned(a_dev, lda, 1, 16), p.fast_b = rows_aligned(b_dev, ldb, 1, 16);
     const hipStream_t s = (hipStream_t)stream;
     with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, s); });
     return ops_launched("ml_fp8_matmul");
@@ -237,13 +237,11 @@ int ml_rms_norm(const void* x_dev, int64_t ldx, const void* residual_dev, int64_
     const long nb = (n + QB - 1) / QB;
     if (ldx < n || (residual_dev && ldr < n) || (h_dev && ldh < n) || (y_dev && ldy < n) || (q_dev && (ldq < n || lds < nb)))
         return ops_fail(ML_ERR_ARG, "ml_rms_norm: a row stride is shorter than its row");
-    if (!(n <= 2048 ? fits((m + 3) / 4, 256) : fits(m, n <= 8192 ? 256 : 1024))) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm: %lld rows of %lld are too many", (long long)m, (long long)n);
+    if (!(n <= 2048 ? fits((m + 3) / 4, 256) : fits(m, n <= 8192 ? 256 : n <= 16384 ? 512 : 1024))) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm: %lld rows of %lld are too many", (long long)m, (long long)n);
     NormParams p{};
     p.x = x_dev, p.residual = residual_dev, p.w = w_dev, p.w_f32 = w_dtype == ML_F32;
     p.m = m, p.n = n, p.ldx = ldx, p.ldr = ldr, p.ldy = q_dev ? ldq : ldy, p.ldh = ldh, p.eps = eps;
     p.y = y_dev, p.h = h_dev, p.q = q_dev, p.scale = scale_dev, p.lds = lds;
-    p.vec = rows_aligned(x_dev, ldx, es, 16) && rows_aligned(residual_dev, ldr, es, 16) && rows_aligned(h_dev, ldh, es, 16) &&
-            rows_aligned(y_dev, ldy, es, 16) && rows_aligned(q_dev, ldq, 1, 8) && ((uintptr_t)w_dev % 16) == 0;
     const hipStream_t s = (hipStream_t)stream;
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -270,8 +268,6 @@ int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int
         NormBackParams p{};
         p.dy = dy_dev, p.h = h_dev, p.w = w_dev, p.dh = dh_dev, p.w_f32 = w_dtype == ML_F32;
         p.m = m, p.n = n, p.ldy = ldy, p.ldh = ldh, p.ldd = ldd, p.ldx = ldx, p.eps = eps, p.dx = dx_dev, p.part = work_dev;
-        p.vec = rows_aligned(dy_dev, ldy, es, 16) && rows_aligned(h_dev, ldh, es, 16) && rows_aligned(dh_dev, ldd, es, 16) &&
-                rows_aligned(dx_dev, ldx, es, 16) && ((uintptr_t)w_dev % 16) == 0;
         with_type(dtype, [&](auto t) { launch_norm_back<decltype(t)>(p, (unsigned)groups, s); });
         const int rc = ops_launched("ml_rms_norm_backward");
         if (rc) return rc;

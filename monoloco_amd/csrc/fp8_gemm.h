@@ -33,17 +33,16 @@ struct GemmParams {
     int bias_dtype;
     void* c;
     long m, n, k, ldc;
-    int fast_a, fast_b;     // rows are 16-byte aligned: whole 16-byte pieces inside a row are loaded as such
-    int vec_c;              // rows of c are 16-byte aligned
+    int fast_a, fast_b;     // rows start on 16 bytes: what the LDS-DMA of the ring wants
 };
 
 // 16 bytes of row `row` at column `col`; what lies behind the matrix is 0 (codes 0 = value 0)
-__device__ __forceinline__ u32x4 load16(const uint8_t* p, long ld, long rows, long k, bool fast, long row, long col) {
+__device__ __forceinline__ u32x4 load16(const uint8_t* p, long ld, long rows, long k, long row, long col) {
     u32x4 v = {0, 0, 0, 0};
     if (row < rows && col < k) {
         const uint8_t* const at = p + row * ld + col;
-        if (fast && col + 16 <= k) {
-            v = *(const u32x4*)at;
+        if (col + 16 <= k) {
+            v = load_any<u32x4>(at);
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -94,9 +93,9 @@ __device__ __forceinline__ void store4(const GemmParams& p, long i, long j, cons
     float x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = v[e] + bias_at(p, j + e);
-    if (p.vec_c && j + 4 <= p.n) {
+    if (j + 4 <= p.n) {
         typedef T t4 __attribute__((ext_vector_type(4)));
-        *(t4*)at = t4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+        store_any(at, t4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]});
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -119,8 +118,8 @@ __global__ __launch_bounds__(256) void fp8_gemm64_kernel(GemmParams p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = (threadIdx.x >> 3) + 32 * i, ch = threadIdx.x & 7;
-            *(u32x4*)(lds[0] + r * QB + ((ch ^ (r & 7)) * 16)) = load16(p.a, p.lda, p.m, p.k, p.fast_a, m0 + r, t * QB + ch * 16);
-            *(u32x4*)(lds[1] + r * QB + ((ch ^ (r & 7)) * 16)) = load16(p.b, p.ldb, p.n, p.k, p.fast_b, n0 + r, t * QB + ch * 16);
+            *(u32x4*)(lds[0] + r * QB + ((ch ^ (r & 7)) * 16)) = load16(p.a, p.lda, p.m, p.k, m0 + r, t * QB + ch * 16);
+            *(u32x4*)(lds[1] + r * QB + ((ch ^ (r & 7)) * 16)) = load16(p.b, p.ldb, p.n, p.k, n0 + r, t * QB + ch * 16);
         }
         __syncthreads();
         const unsigned xa = sa[t], xb = sb[t];
@@ -268,7 +267,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         for (int u = tid; u < ROWS * 8; u += 256) {
             const int half = u / (ROWS * 4), v = u - half * ROWS * 4, r = v >> 2, ch = v & 3;
             const long col = k0 + half * 64 + ch * 16;
-            const u32x4 x = r < BN ? load16(p.b, p.ldb, p.n, p.k, true, n0 + r, col) : load16(p.a, p.lda, p.m, p.k, true, m0 + r - BN, col);
+            const u32x4 x = r < BN ? load16(p.b, p.ldb, p.n, p.k, n0 + r, col) : load16(p.a, p.lda, p.m, p.k, m0 + r - BN, col);
             *(u32x4*)(smem + half * SLOT + r * 64 + ((ch ^ ((r >> 2) & 3)) * 16)) = x;
         }
         __syncthreads();
@@ -388,7 +387,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
     char* const scr = smem + w * PASS * 32 * PITCH;
     typedef T t4 __attribute__((ext_vector_type(4)));
     typedef T tv __attribute__((ext_vector_type(EV)));
-    const bool inside = m0 + BM <= p.m && n0 + BN <= p.n && p.vec_c;
+    const bool inside = m0 + BM <= p.m && n0 + BN <= p.n;
     const long row0 = m0 + wm * 32 * NJ, col0 = n0 + wn * 32 * NI;
 #pragma unroll
     for (int j0 = 0; j0 < NJ; j0 += PASS) {
@@ -422,7 +421,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
 #pragma unroll
                 for (int x = 0; x < 8; ++x)
                     if (u + x < UNITS) {
-                        *(tv*)out = v[x];
+                        store_any(out, v[x]);
                         out += by;
                     }
             }
@@ -434,8 +433,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
                 const tv v = *(const tv*)(from + u * STEP * PITCH);
                 if (row < p.m && col < p.n) {
                     T* const out = (T*)p.c + row * p.ldc + col;
-                    if (p.vec_c && col + EV <= p.n) {
-                        *(tv*)out = v;
+                    if (col + EV <= p.n) {
+                        store_any(out, v);
                     } else {
 #pragma unroll
                         for (int e = 0; e < EV; ++e)
@@ -456,7 +455,7 @@ __device__ __forceinline__ float from_acc(float a) {
 }
 
 // ---- the streaming kernel: 256 x 256 tiles, 16-bit results, a workgroup per CU that walks tiles without a pause ----------------------
-// The ring kernel's steps with 4 x 4 matrix tiles per wave, for k a multiple of 128 from 512 on, n a multiple of 8, rows of c on 16 bytes.  There a tile of 16 steps spent 17000 of
+// The ring kernel's steps with 4 x 4 matrix tiles per wave, for k a multiple of 128 from 512 on, n a multiple of 8.  There a tile of 16 steps spent 17000 of
 // its 38000 cycles outside its products (start and addresses 5000, first latency 3600, epilogue 8000).  Here the last four steps of a tile
 // already request the first four of the next one; the next tile's scales and bias are loaded in front of the epilogue and written to LDS
 // behind it; and the epilogue needs no LDS: v_permlane32_swap joins the 4 + 4 columns of two lanes into 16 bytes of a row, stored
@@ -663,7 +662,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void f
                         }
                         const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false), y = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
                         const u32x4 q = {(unsigned)x[0], (unsigned)y[0], (unsigned)x[1], (unsigned)y[1]};
-                        if (!EDGE || (j * 32 < rows && i * 32 + h * 16 < cols)) *(u32x4*)(out0 + (long)j * 32 * p.ldc + i * 32 + h * 16) = q;
+                        if (!EDGE || (j * 32 < rows && i * 32 + h * 16 < cols)) store_any(out0 + (long)j * 32 * p.ldc + i * 32 + h * 16, q);
                     }
             }
         };
@@ -711,8 +710,8 @@ __global__ __launch_bounds__(512) void fp8_gemm_rows_kernel(GemmParams p) {
         const long r = min((long)(i * 16 + lr), p.m - 1);
         sa[i] = p.sa + (p.a_tile ? r / QB : r) * p.ldsa;
     }
-    auto frag = [&](const uint8_t* x, long ld, long rows, bool fast, long row, long col) {
-        const u32x4 u = load16(x, ld, rows, p.k, fast, row, col), v = load16(x, ld, rows, p.k, fast, row, col + 16);
+    auto frag = [&](const uint8_t* x, long ld, long rows, long row, long col) {
+        const u32x4 u = load16(x, ld, rows, p.k, row, col), v = load16(x, ld, rows, p.k, row, col + 16);
         return i32x8{(int)u[0], (int)u[1], (int)u[2], (int)u[3], (int)v[0], (int)v[1], (int)v[2], (int)v[3]};
     };
     f32x4 acc[MT] = {};
@@ -722,11 +721,11 @@ __global__ __launch_bounds__(512) void fp8_gemm_rows_kernel(GemmParams p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long b = t + u * WAVES, col = b * QB + lg * 32;    // (behind the last block: zeros, scale 1)
-            fb[u] = frag(p.b, p.ldb, p.n, p.fast_b, n0 + lr, col);
+            fb[u] = frag(p.b, p.ldb, p.n, n0 + lr, col);
             xb[u] = b < kb ? sb[b] : 127;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                fa[u][i] = frag(p.a, p.lda, p.m, p.fast_a, i * 16 + lr, col);
+                fa[u][i] = frag(p.a, p.lda, p.m, i * 16 + lr, col);
                 xa[u][i] = b < kb ? sa[i][b] : 127;
             }
         }

@@ -17,7 +17,6 @@ struct QuantParams {
     uint8_t* scale_t;   // (n, mb) or (nb, mb), row stride ldst
     long ldqt, ldst;
     float* colsum;      // (mb, n): column sums of every 128 rows, or null
-    int vec, vecq, vecqt;
 };
 
 // rows only: 16 lanes per block of 128, no LDS
@@ -28,12 +27,12 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantParams p) {
     if (u >= units) return;   // (whole groups of 16 lanes)
     const long row = u / nb, b = u - row * nb, c = b * QB + (threadIdx.x & 15) * 8;
     float x[8];
-    load8((const T*)p.x + row * p.ldx + c, p.n - c, p.vec, x);
+    load8((const T*)p.x + row * p.ldx + c, p.n - c, x);
     unsigned a = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) a = max(a, absbits(x[i]));
     const unsigned byte = scale_byte(max16(a));
-    if (c < p.n) store_codes8(p.q + row * p.ldq + c, p.n - c, p.vecq, codes8(x, byte));
+    if (c < p.n) store_codes8(p.q + row * p.ldq + c, p.n - c, codes8(x, byte));
     if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + b] = (uint8_t)byte;
 }
 
@@ -53,7 +52,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void q
     Vec8<T> x[8];
     unsigned rmax[8], colmax[8] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = load_raw8((const T*)p.x + (r0 + i) * p.ldx + c0, r0 + i < p.m ? p.n - c0 : 0, p.vec);
+    for (int i = 0; i < 8; ++i) x[i] = load_raw8((const T*)p.x + (r0 + i) * p.ldx + c0, r0 + i < p.m ? p.n - c0 : 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         rmax[i] = 0;
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void q
                 v[2 + d] = odd ? keep : got;
             }
             const long row = r0 + i + (odd ? 1 : 0);
-            if (row < p.m && cc < p.n) store_codes16(p.q + row * p.ldq + cc, p.n - cc, p.vecq, v);
+            if (row < p.m && cc < p.n) store_codes16(p.q + row * p.ldq + cc, p.n - cc, v);
         }
         if (p.tile && threadIdx.x == 0) p.scale[bi * p.lds + bj] = (uint8_t)tb;
     }
@@ -140,7 +139,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void q
         for (int k = 0; k < 4; ++k) {
             const int c = (threadIdx.x >> 3) + 32 * k, ch = threadIdx.x & 7;
             const long rt = bj * QB + c, ct = bi * QB + ch * 16;
-            if (rt < p.n && ct < p.m) store_codes16(p.qt + rt * p.ldqt + ct, p.m - ct, p.vecqt, *(const u32x4*)(tq + c * QB + ((ch ^ ((c >> 3) & 7)) * 16)));
+            if (rt < p.n && ct < p.m) store_codes16(p.qt + rt * p.ldqt + ct, p.m - ct, *(const u32x4*)(tq + c * QB + ((ch ^ ((c >> 3) & 7)) * 16)));
         }
     }
 }

@@ -7,7 +7,7 @@
 // A row stays in registers between its reduction and its output, so everything is read once.  A lane owns chunks of 8 consecutive
 // elements (one 16-byte access of a 2-byte type; 16 neighbouring lanes = one block of 128 of the 8-bit output, whose maximum is
 // four DPP rotations).  WPR = waves per row, NV = chunks per lane: a row of up to 2048 elements is one wave's (no LDS, no barrier;
-// four rows per workgroup), longer ones take 4 or 16 waves; NV = 0 streams rows beyond 32768
+// four rows per workgroup), longer ones take 4, 8 or 16 waves; NV = 0 streams rows beyond 32768
 // elements (backward: 16384) from memory twice.
 #pragma once
 #include "block8.h"
@@ -26,7 +26,6 @@ struct NormParams {
     uint8_t* q;             // (m, n) codes, or null
     uint8_t* scale;         // (m, blocks), row stride lds
     long lds;
-    int vec;                // every operand's rows are 16-byte aligned (q: 8)
 };
 
 template <int WPR>
@@ -47,16 +46,16 @@ __device__ __forceinline__ float row_sum(float x, float* red) {
 __device__ __forceinline__ float row_rstd(float ss, long n, float eps) { return (float)(1.0 / sqrt((double)ss / (double)n + (double)eps)); }
 
 template <typename T>
-__device__ __forceinline__ void load_weight8(const void* w, int w_f32, long c, long n, bool vec, float (&x)[8]) {
-    if (w_f32) load8((const float*)w + c, n - c, vec, x);
-    else load8((const T*)w + c, n - c, vec, x);
+__device__ __forceinline__ void load_weight8(const void* w, int w_f32, long c, long n, float (&x)[8]) {
+    if (w_f32) load8((const float*)w + c, n - c, x);
+    else load8((const T*)w + c, n - c, x);
 }
 
 // one chunk's output
 template <typename T, bool OUT8>
 __device__ __forceinline__ void norm_out(const NormParams& p, long row, long c, const float (&h)[8], float rstd) {
     float wv[8], y[8];
-    load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
+    load_weight8<T>(p.w, p.w_f32, c, p.n, wv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = h[i] * rstd * wv[i];
     if (OUT8) {
@@ -65,20 +64,20 @@ __device__ __forceinline__ void norm_out(const NormParams& p, long row, long c, 
         for (int i = 0; i < 8; ++i) a = max(a, c + i < p.n ? absbits(y[i]) : 0u);
         const unsigned byte = scale_byte(max16(a));
         if (c < p.n) {
-            store_codes8(p.q + row * p.ldy + c, p.n - c, p.vec, codes8(y, byte));
+            store_codes8(p.q + row * p.ldy + c, p.n - c, codes8(y, byte));
             if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + c / QB] = (uint8_t)byte;
         }
     } else if (c < p.n) {
-        store8((T*)p.y + row * p.ldy + c, p.n - c, p.vec, y);
+        store8((T*)p.y + row * p.ldy + c, p.n - c, y);
     }
 }
 
 template <typename T>
 __device__ __forceinline__ void norm_in(const NormParams& p, long row, long c, float (&h)[8]) {
-    load8((const T*)p.x + row * p.ldx + c, p.n - c, p.vec, h);
+    load8((const T*)p.x + row * p.ldx + c, p.n - c, h);
     if (p.residual) {
         float r[8];
-        load8((const T*)p.residual + row * p.ldr + c, p.n - c, p.vec, r);
+        load8((const T*)p.residual + row * p.ldr + c, p.n - c, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[i] += r[i];
     }
@@ -104,7 +103,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_kernel(Nor
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const long c = lane * 8 + j * STEP;
-            if (p.h && c < p.n) store8((T*)p.h + row * p.ldh + c, p.n - c, p.vec, h[j]);
+            if (p.h && c < p.n) store8((T*)p.h + row * p.ldh + c, p.n - c, h[j]);
             norm_out<T, OUT8>(p, row, c, h[j], rstd);
         }
     } else {   // long rows: once for the sum, once for the output
@@ -118,7 +117,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_kernel(Nor
         const float rstd = row_rstd(row_sum<WPR>(ss, red), p.n, p.eps);
         for (long c = lane * 8; c < end; c += STEP) {
             norm_in<T>(p, row, c, h);
-            if (p.h && c < p.n) store8((T*)p.h + row * p.ldh + c, p.n - c, p.vec, h);
+            if (p.h && c < p.n) store8((T*)p.h + row * p.ldh + c, p.n - c, h);
             norm_out<T, OUT8>(p, row, c, h, rstd);
         }
     }
@@ -134,7 +133,6 @@ struct NormBackParams {
     float eps;
     void* dx;         // (m, n)
     float* part;      // (groups, n) partial sums of dw
-    int vec;
 };
 
 // A workgroup takes rows g, g + groups, ...; a lane keeps its columns' part of dw in registers over all of them.  The partial sums
@@ -155,15 +153,15 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
         constexpr bool AHEAD = NV * (int)sizeof(T) <= 4;
         float dw[NV][8] = {}, wv[NV][8];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) load_weight8<T>(p.w, p.w_f32, lane * 8 + j * STEP, p.n, p.vec, wv[j]);
+        for (int j = 0; j < NV; ++j) load_weight8<T>(p.w, p.w_f32, lane * 8 + j * STEP, p.n, wv[j]);
         struct Row { Vec8<T> h[NV], g[NV], d[NV]; };
         auto fetch = [&](Row& r, long row) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const long c = lane * 8 + j * STEP;
-                r.h[j] = load_raw8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec);
-                r.g[j] = load_raw8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec);
-                if (p.dh) r.d[j] = load_raw8((const T*)p.dh + row * p.ldd + c, p.n - c, p.vec);
+                r.h[j] = load_raw8((const T*)p.h + row * p.ldh + c, p.n - c);
+                r.g[j] = load_raw8((const T*)p.dy + row * p.ldy + c, p.n - c);
+                if (p.dh) r.d[j] = load_raw8((const T*)p.dh + row * p.ldd + c, p.n - c);
             }
         };
         Row now;
@@ -201,7 +199,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
                     d[i] = rstd * (g * wv[j][i] - h * k);
                     if (p.dh) d[i] += vget(now.d[j], i);
                 }
-                if (c < p.n) store8((T*)p.dx + row * p.ldx + c, p.n - c, p.vec, d);
+                if (c < p.n) store8((T*)p.dx + row * p.ldx + c, p.n - c, d);
             }
             if (AHEAD) now = next;
         }
@@ -231,9 +229,9 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
         for (long row = blockIdx.x; row < p.m; row += gridDim.x, first = false) {
             float h[8], g[8], wv[8], ss = 0.0f, gh = 0.0f;
             for (long c = lane * 8; c < p.n; c += STEP) {
-                load8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec, h);
-                load8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec, g);
-                load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
+                load8((const T*)p.h + row * p.ldh + c, p.n - c, h);
+                load8((const T*)p.dy + row * p.ldy + c, p.n - c, g);
+                load_weight8<T>(p.w, p.w_f32, c, p.n, wv);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     ss += h[i] * h[i];
@@ -246,17 +244,17 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
             const float k = rstd * rstd * (gh * inv_n);
             for (long c = lane * 8; c < p.n; c += STEP) {
                 float d[8];
-                load8((const T*)p.h + row * p.ldh + c, p.n - c, p.vec, h);
-                load8((const T*)p.dy + row * p.ldy + c, p.n - c, p.vec, g);
-                load_weight8<T>(p.w, p.w_f32, c, p.n, p.vec, wv);
-                if (p.dh) load8((const T*)p.dh + row * p.ldd + c, p.n - c, p.vec, d);
+                load8((const T*)p.h + row * p.ldh + c, p.n - c, h);
+                load8((const T*)p.dy + row * p.ldy + c, p.n - c, g);
+                load_weight8<T>(p.w, p.w_f32, c, p.n, wv);
+                if (p.dh) load8((const T*)p.dh + row * p.ldd + c, p.n - c, d);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if (c + i < p.n) part[c + i] = (first ? 0.0f : part[c + i]) + g[i] * (h[i] * rstd);
                     const float v = rstd * (g[i] * wv[i] - h[i] * k);
                     d[i] = p.dh ? v + d[i] : v;
                 }
-                store8((T*)p.dx + row * p.ldx + c, p.n - c, p.vec, d);
+                store8((T*)p.dx + row * p.ldx + c, p.n - c, d);
             }
         }
     }

@@ -350,7 +350,7 @@ def test_linear_shapes_views_and_modes(cuda_device):
 
 # -------------------------------------------------------------------------------------------------------------------- norm
 NORMS = [(1, 1), (1, 34), (3, 127), (5, 129), (4, 512), (6, 513), (7, 1024), (331, 1001), (3, 1025), (2, 2048), (3, 2050), (2, 4097), (2, 8192),
-         (2, 9001), (1, 32768), (2, 33001)]
+         (2, 9001), (2, 16384), (2, 16386), (1, 32768), (2, 33001)]
 
 
 @pytest.mark.parametrize('m,n', NORMS)
@@ -487,3 +487,58 @@ def test_block_on_a_stream_and_in_a_graph(cuda_device):
         torch.cuda.synchronize()
         got = [t.clone() for t in out]
         assert all(torch.equal(a, b) for a, b in zip(got, block()))
+
+
+# ------------------------------------------------------------------------------------------- the operators together, in training
+def test_residual_block_trains(cuda_device):
+    """Three steps of x -> norm(x + r) -> linear -> relu -> linear, + h, with AdamW in 8 bits: every operator's results against its plain
+    64-bit form on the inputs it had, so that one operator's rounding is never another's error."""
+    from monoloco_amd.train import AdamW
+    m, n, k = 200, 192, 320
+    g = torch.Generator().manual_seed(5)
+    w, w1, b1, w2 = (torch.nn.Parameter(t.to(cuda_device)) for t in (1 + 0.1 * torch.randn(n, generator=g), torch.randn((k, n), generator=g) / 14,
+                                                                     0.1 * torch.randn(k, generator=g), torch.randn((n, k), generator=g) / 18))
+    params = [w, w1, b1, w2]
+    opt = AdamW(params, lr=1e-2, weight_decay=0.1, state_bits=8, seed=11)
+    f32 = torch.float32
+    for it in range(3):
+        x, r, want = (data(100 * it + i, m, n, f32, 0.2).to(cuda_device) for i in range(3))
+        for t in params:
+            t.grad = None
+        y, h = fp8.rms_norm(x, w, residual=r)
+        a = fp8.linear(y, w1, b1)
+        c = torch.relu(a)
+        d = fp8.linear(c, w2)
+        out = d + h
+        kept = [t.detach().cpu() for t in (y, c, d)]
+        for t in (y, h, a, c, d):
+            t.retain_grad()
+        ((out - want) ** 2).sum().backward()
+        wy, _ = R.rms_norm(x.cpu(), w.detach().cpu(), r.cpu(), 1e-6)
+        assert bool(((kept[0].double() - wy).abs() <= 71 * U * wy.abs()).all())
+        close_product(a.detach(), R.rounded(kept[0]), R.rounded(w1.detach().cpu(), True), b1.detach().cpu(), f32)
+        close_product(d.detach(), R.rounded(kept[1]), R.rounded(w2.detach().cpu(), True), None, f32)
+        dd, da = d.grad.cpu(), a.grad.cpu()
+        close_product(c.grad, R.rounded(dd), R.rounded(w2.detach().cpu(), True).t().contiguous(), None, f32)
+        close_product(w2.grad, R.rounded(dd.t().contiguous()), R.rounded(kept[1].t().contiguous()), None, f32)
+        close_product(y.grad, R.rounded(da), R.rounded(w1.detach().cpu(), True).t().contiguous(), None, f32)
+        close_product(w1.grad, R.rounded(da.t().contiguous()), R.rounded(kept[0].t().contiguous()), None, f32)
+        assert bool(((b1.grad.cpu().double() - da.double().sum(0)).abs() <= (m + 64) * U * da.double().abs().sum(0)).all())
+        # (x needs no gradient here: the norm's is the weight's)
+        _, ew, _, aw = R.rms_norm_backward(y.grad.cpu(), h.detach().cpu(), w.detach().cpu(), None, 1e-6)
+        assert bool(((w.grad.cpu().double() - ew).abs() <= (m + 71) * U * aw).all())
+        before = [t.detach().cpu().double() for t in params]
+        state = [{key: v.clone() for key, v in opt.state[t].items() if isinstance(v, torch.Tensor)} if opt.state[t] else None for t in params]
+        opt.step()
+        for t, p0, s0 in zip(params, before, state):
+            num = p0.numel()
+
+            def value(key, row):
+                if s0 is None:
+                    return torch.zeros(p0.shape, dtype=torch.float64)
+                sc = R.scale_values(s0['scales'].view(torch.uint8)[row].cpu()).repeat_interleave(128)[:num]
+                return (s0[key].cpu().float().double().reshape(-1) * sc).view(p0.shape)
+
+            m0, r0 = value('exp_avg', 0), value('exp_avg_sq', 1)
+            p1, _, _, am, size = R.adamw(p0, t.grad.cpu().double(), m0, r0 * r0, it + 1, 1e-2, (0.9, 0.999), 1e-8, 0.1)
+            assert bool(((t.detach().cpu().double() - p1).abs() <= 16 * U * size * am + 4 * U * p0.abs() + U * p1.abs()).all())
