@@ -52,8 +52,8 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
 //   m <= 32 rows (fp32 results: 64): the waves of a workgroup share k.  4096 x 4096, m = 32: 10.5 against 12.9 with 64 x 64 tiles; m = 64:
 //     16.4 against 13.1, fp32 18.1 against 24.6.
 //   The ring wants rows that start on 16 bytes and offsets inside a tile below 2^32; everything else takes the plain 64 x 64 kernel.
-//   64 x 64 tiles while they fit the CUs once (or, k <= 2048, twice): 512 x 1024 x 1024 6.1 against 7.9 with 128 x 128; 2048 x 1024 x 1024
-//     7.7 against 8.4; 384 x 4096 x 4096 (384 tiles) 22.4 against 18.5.  fp32: while the 128 x 128 tiles are fewer than the CUs.
+//   64 x 64 tiles while they fit the CUs once (or, k <= 2048, twice): 512 x 1024 x 1024 5.7 against 7.9 with 128 x 128; 2048 x 1024 x 1024
+//     7.0 against 8.4; 384 x 4096 x 4096 (384 tiles) 22.4 against 18.5.  fp32: while the 128 x 128 tiles are fewer than the CUs.
 //   256 x 256 tiles (16-bit results) once they are more than the CUs, or k >= 2048 and 160 of them: 16384 x 1024 x 1024 (256 tiles) 26.9
 //     against 24.6 with 128 x 128, 32768 x 1024 x 1024 44.7 against 48.9; 2048 x 4096 x 4096 (128) 47.1 against 40.9, 4096^3 (256) 59.7
 //     against 77.9; below k = 1024 a tile's start and end outweigh its steps.
@@ -64,13 +64,13 @@ void launch_gemm(const GemmParams& p, hipStream_t s) {
     auto across = [&](long t) { return (p.m + t - 1) / t * ((p.n + t - 1) / t); };
     const long t256 = across(256), t128 = across(128), t64 = across(64);
     auto tiles = [](long size, int t) { return (int)((size + t - 1) / t); };
-    const unsigned g16 = (unsigned)((p.n + 15) / 16);
-    if (p.m <= 16) {
-        fp8_gemm_rows_kernel<T, 1, 4><<<g16, 512, 0, s>>>(p);
-    } else if (p.m <= 32) {
-        fp8_gemm_rows_kernel<T, 2, 2><<<g16, 512, 0, s>>>(p);
-    } else if (!HALF && p.m <= 64) {
-        if constexpr (!HALF) fp8_gemm_rows_kernel<T, 4, 2><<<g16, 512, 0, s>>>(p);
+    const long g16 = (p.n + 15) / 16;
+    if (p.m <= 16 && fits(g16, 512)) {
+        fp8_gemm_rows_kernel<T, 1, 4><<<(unsigned)g16, 512, 0, s>>>(p);
+    } else if (p.m <= 32 && fits(g16, 512)) {
+        fp8_gemm_rows_kernel<T, 2, 2><<<(unsigned)g16, 512, 0, s>>>(p);
+    } else if (!HALF && p.m <= 64 && fits(g16, 512)) {
+        if constexpr (!HALF) fp8_gemm_rows_kernel<T, 4, 2><<<(unsigned)g16, 512, 0, s>>>(p);
     } else if (!ring) {
         fp8_gemm64_kernel<T><<<(unsigned)t64, 256, 0, s>>>(p);
     } else if (HALF && p.k >= 1024 && (t256 > 256 || (t256 >= 160 && p.k >= 2048))) {

@@ -249,6 +249,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
                 if (tid + 256 * i < ROWS && 4 * j < have) *(unsigned*)(slds + (tid + 256 * i) * G8_SPITCH + 4 * j) = v[i][j];
     };
 
+    // everything outstanding, by the builtin: hipcc has to know that fill_scales' loads are done (threads without a row never use theirs, and
+    // it would wait for them, and with them for every request, inside the steps)
+    auto drain = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0);
+        asm volatile("" ::: "memory");
+    };
+
     f32x16 acc[NI][NJ];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
@@ -300,7 +308,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         const float b = tid < BN ? bias_at(p, n0 + tid) : 0.0f;
         fill_scales(0);   // (its wait is the first steps', too: their latencies overlap)
         if (tid < BN) bias[tid] = b;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        drain();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -347,7 +355,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         auto chunk = [&](int s) {   // in front of the first step of the next 32 blocks: nobody reads the last ones' scales any more
             if ((s & (2 * G8_CHUNK - 1)) == 0 && s > 0) {
                 fill_scales(s >> 1);
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                drain();
                 __builtin_amdgcn_s_barrier();
                 read_scales(s >> 1);
             }

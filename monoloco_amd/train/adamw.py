@@ -82,17 +82,15 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
         _need(state_bits in (8, 32), "AdamW: moments have 8 or 32 bits, not %r", state_bits)
         _need(lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas), "AdamW: lr, eps and weight_decay are not negative, betas are in [0, 1)")
-        self.state_bits, self.seed = state_bits, int(seed)
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=int(seed)))
 
-    def _state(self, p):
+    def _state(self, p, bits):
         s = self.state[p]
         if not s:
             s['step'] = 0
-            dt = torch.float32 if self.state_bits == 32 else CODES
             for key in ('exp_avg', 'exp_avg_sq'):
-                s[key] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(dt)
-            if self.state_bits == 8:
+                s[key] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(torch.float32 if bits == 32 else CODES)
+            if bits == 8:
                 s['scales'] = state_scales(p.numel(), p.device)
         return s
 
@@ -103,29 +101,40 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            calls = {}
+            calls, bits = {}, group['state_bits']
             for p in group['params']:
                 if p.grad is None:
                     continue
                 _need(not p.grad.is_sparse, "AdamW: sparse gradients are not supported")
-                s = self._state(p)
+                s = self._state(p, bits)
                 calls.setdefault((p.device, p.dtype, s['step'] + 1), []).append((p, s))
             for (_, _, step), found in calls.items():
                 adamw_step([p for p, _ in found], [p.grad for p, _ in found], [s['exp_avg'] for _, s in found], [s['exp_avg_sq'] for _, s in found],
-                           [s['scales'] for _, s in found] if self.state_bits == 8 else None, step=step, lr=float(group['lr']), betas=group['betas'],
-                           eps=group['eps'], weight_decay=group['weight_decay'], seed=self.seed)
+                           [s['scales'] for _, s in found] if bits == 8 else None, step=step, lr=float(group['lr']), betas=group['betas'],
+                           eps=group['eps'], weight_decay=group['weight_decay'], seed=group['seed'])
                 for _, s in found:
                     s['step'] = step
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the moments keep the types they were saved in (the base class casts them to the parameters')."""
+        """As torch's, but the moments keep the types they were saved in (the base class casts them to the parameters').  A state_dict of
+        ``torch.optim.AdamW`` loads, too (moments in 32 bits)."""
+        own = [{k: g[k] for k in ('state_bits', 'seed')} for g in self.param_groups]
+        saved_groups = state_dict['param_groups']
+        for mine, saved in zip(own, saved_groups):
+            bits = saved.get('state_bits', 32)
+            _need(bits == mine['state_bits'], "AdamW: the saved moments have %d bits, this optimizer's %d", bits, mine['state_bits'])
         super().load_state_dict(state_dict)
-        ids = [i for g in state_dict['param_groups'] for i in g['params']]
-        params = [p for g in self.param_groups for p in g['params']]
-        for i, p in zip(ids, params):
+        ids = [i for g in saved_groups for i in g['params']]
+        for g, mine in zip(self.param_groups, own):
+            for k, v in mine.items():
+                g.setdefault(k, v)
+        for i, p in zip(ids, [p for g in self.param_groups for p in g['params']]):
             saved = state_dict['state'].get(i)
             if saved:
-                eight = saved['exp_avg'].dtype == CODES
-                _need(eight == (self.state_bits == 8), "AdamW: the saved moments have %d bits, this optimizer's %d", 8 if eight else 32, self.state_bits)
-                self.state[p] = {k: v.detach().to(p.device).clone() if isinstance(v, torch.Tensor) else v for k, v in saved.items()}
+                state = {'step': int(saved['step'])}
+                for k in ('exp_avg', 'exp_avg_sq', 'scales'):
+                    if k in saved:
+                        v = saved[k].detach().to(p.device).clone()
+                        state[k] = v.float() if v.dtype in DTYPES else v
+                self.state[p] = state

@@ -249,6 +249,29 @@ def test_optimizer_8_bits_state_dict(cuda_device):
     assert torch.equal(p, p2)
     with pytest.raises(ValueError):
         AdamW([p2], state_bits=32).load_state_dict(o.state_dict())
+    twin = copy.deepcopy(o)                     # a copy keeps what it needs for its next step
+    q = twin.param_groups[0]['params'][0]
+    q.grad = p.grad.clone()
+    o.step(), twin.step()
+    assert torch.equal(p, q)
+
+
+def test_optimizer_takes_over_from_torch(cuda_device):
+    g0 = torch.Generator().manual_seed(9)
+    p = torch.nn.Parameter(torch.randn(300, generator=g0).to(cuda_device))
+    q = torch.nn.Parameter(p.detach().clone())
+    a, b = torch.optim.AdamW([p], lr=1e-2), AdamW([q], lr=1e-2)
+    for it in range(4):
+        g = torch.randn(300, generator=g0).to(cuda_device)
+        if it == 2:
+            q.data.copy_(p.data)
+            b.load_state_dict(copy.deepcopy(a.state_dict()))
+            assert b.state[q]['step'] == 2 and b.param_groups[0]['state_bits'] == 32
+        for t, o in ((p, a), (q, b)):
+            t.grad = g.clone()
+            o.step()
+    # two steps of the same formula in fp32 from the same state: (16 u * 1e-2 + 4 u |p|) each, on both sides
+    assert float((p - q).abs().max()) <= 4 * (16 * U * 1e-2 * 4 + 4 * U * 5)
 
 
 def test_module_sees_the_step(cuda_device):

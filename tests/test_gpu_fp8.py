@@ -217,6 +217,10 @@ def test_matmul_many_tiles(cuda_device, m, n, k, bias, dtype):
     assert bool((err <= tol)[fine].all())
     assert float(err[fine].norm()) <= (3.5e-4 + half(dtype)) * float(want[fine].norm())
     assert torch.equal(c, fp8.matmul(wa, sa.view(E8), wb, sb.view(E8), bias=bv, out_dtype=dtype))
+    big = torch.full((m + 2, n + 5), 7.0, dtype=dtype, device=cuda_device)        # rows at odd addresses, nothing around them written
+    assert torch.equal(fp8.matmul(wa, sa.view(E8), wb, sb.view(E8), bias=bv, out=big[1:-1, 3:3 + n]), c)
+    big[1:-1, 3:3 + n] = 7.0
+    assert bool((big == 7.0).all())
 
 
 def test_matmul_views_pads_and_out(cuda_device):
@@ -487,6 +491,35 @@ def test_block_on_a_stream_and_in_a_graph(cuda_device):
         torch.cuda.synchronize()
         got = [t.clone() for t in out]
         assert all(torch.equal(a, b) for a, b in zip(got, block()))
+
+
+def test_training_step_in_a_graph(cuda_device):
+    """Norm and linear, forward and backward, captured (no eager graph of the leaves alive) and replayed with eager work in between."""
+    m, n, k = 96, 160, 144
+    w, w1, b1 = (t.to(cuda_device) for t in (1 + 0.1 * data(1, 1, n, torch.float32)[0], data(2, k, n, torch.float32, 0.1) / 12, data(3, 1, k, torch.float32)[0]))
+    x, r, dy = (data(s, m, n if s < 6 else k, torch.bfloat16).to(cuda_device) for s in (4, 5, 6))
+
+    def step():
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, r, w, w1, b1)]
+        y, h = fp8.rms_norm(leaves[0], leaves[2], residual=leaves[1])
+        a = fp8.linear(y, leaves[3], leaves[4])
+        return [a.detach()] + list(torch.autograd.grad((a, h), leaves, (dy, torch.ones_like(h))))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (20, 30, 40):
+        x.copy_(data(seed, m, n, torch.bfloat16).to(cuda_device))
+        dy.copy_(data(seed + 1, m, k, torch.bfloat16).to(cuda_device))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
 # ------------------------------------------------------------------------------------------- the operators together, in training
