@@ -312,6 +312,25 @@ def test_linear(cuda_device, m, n, k, dtype):
         assert torch.equal(got, want)
 
 
+def test_linear_mixed_types(cuda_device):
+    """bf16 rows, an fp32 weight and an fp16 bias: each result in its operand's type, from the kernels of that type."""
+    m, n, k = 140, 130, 260
+    x, w, b, dy = data(1, m, k, torch.bfloat16), data(2, n, k, torch.float32, 0.1), data(3, 1, n, torch.float16)[0], data(4, m, n, torch.bfloat16)
+    xs, ws, bs = (t.to(cuda_device).requires_grad_(True) for t in (x, w, b))
+    y = fp8.linear(xs, ws, bs)
+    dx, dw, db = torch.autograd.grad(y, (xs, ws, bs), dy.to(cuda_device))
+    wq = R.rounded(w, True)
+    close_product(y.detach(), R.rounded(x), wq, b, torch.bfloat16)
+    close_product(dx, R.rounded(dy), wq.t().contiguous(), None, torch.bfloat16)
+    close_product(dw, R.rounded(dy.t().contiguous()), R.rounded(x.t().contiguous()), None, torch.float32)
+    assert db.dtype == torch.float16
+    want, mag = dy.double().sum(0), dy.double().abs().sum(0)
+    assert bool(((db.cpu().double() - want).abs() <= (m + 64) * U * mag + half(torch.float16) * want.abs() + 2.0 ** -25).all())
+    with pytest.raises(RuntimeError):                     # once differentiable: a second derivative is refused, not zero
+        g, = torch.autograd.grad(fp8.linear(xs, ws, bs).float().square().sum(), xs, create_graph=True)
+        g.float().sum().backward()
+
+
 def test_linear_gradient_against_differences(cuda_device):
     """The loss sum(y * g) is piecewise constant in 8 bits; over a step that is large against the rounding its difference is the
     gradient's: a direction d of size 2 moves it by sum(dx * d), off by at most the roundings of x and g on both ends (2^-4 each)."""
