@@ -54,9 +54,10 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
 //   The ring wants rows that start on 16 bytes and offsets inside a tile below 2^32; everything else takes the plain 64 x 64 kernel.
 //   64 x 64 tiles while they fit the CUs once (or, k <= 2048, twice): 512 x 1024 x 1024 5.7 against 7.9 with 128 x 128; 2048 x 1024 x 1024
 //     7.0 against 8.4; 384 x 4096 x 4096 (384 tiles) 22.4 against 18.5.  fp32: while the 128 x 128 tiles are fewer than the CUs.
-//   256 x 256 tiles (16-bit results) once they are more than the CUs, or k >= 2048 and 160 of them: 16384 x 1024 x 1024 (256 tiles) 26.9
+//   256 x 256 tiles once they are more than the CUs, or k >= 2048 and 160 of them: 16384 x 1024 x 1024 (256 tiles) 26.9
 //     against 24.6 with 128 x 128, 32768 x 1024 x 1024 44.7 against 48.9; 2048 x 4096 x 4096 (128) 47.1 against 40.9, 4096^3 (256) 59.7
-//     against 77.9; below k = 1024 a tile's start and end outweigh its steps.
+//     against 77.9; below k = 1024 a tile's start and end outweigh its steps.  fp32: 2560 x 4096 x 4096 (160) 97 against 98, 4096^3 114 against
+//     133, 8192^3 856 against 986.
 template <typename T>
 void launch_gemm(const GemmParams& p, hipStream_t s) {
     constexpr bool HALF = sizeof(T) == 2;
@@ -73,11 +74,13 @@ void launch_gemm(const GemmParams& p, hipStream_t s) {
         if constexpr (!HALF) fp8_gemm_rows_kernel<T, 4, 2><<<(unsigned)g16, 512, 0, s>>>(p);
     } else if (!ring) {
         fp8_gemm64_kernel<T><<<(unsigned)t64, 256, 0, s>>>(p);
-    } else if (HALF && p.k >= 1024 && (t256 > 256 || (t256 >= 160 && p.k >= 2048))) {
+    } else if (p.k >= 1024 && (t256 > 256 || (t256 >= 160 && p.k >= 2048))) {
+        bool streamed = false;
         if constexpr (HALF) {
-            if (p.k % QB == 0 && p.n % 8 == 0) fp8_gemm_stream_kernel<T><<<(unsigned)(t256 < 256 ? t256 : 256), 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
-            else fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
+            streamed = p.k % QB == 0 && p.n % 8 == 0;
+            if (streamed) fp8_gemm_stream_kernel<T><<<(unsigned)(t256 < 256 ? t256 : 256), 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
         }
+        if (!streamed) fp8_gemm_ring_kernel<T, 4, 4><<<(unsigned)t256, 256, 0, s>>>(p, tiles(p.m, 256), tiles(p.n, 256));
     } else if (HALF ? t64 <= (p.k <= 2048 ? 512 : 256) : t128 < 256) {
         fp8_gemm_ring_kernel<T, 1, 1><<<(unsigned)t64, 256, 0, s>>>(p, tiles(p.m, 64), tiles(p.n, 64));
     } else {

@@ -55,15 +55,13 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* p, long ld, long rows, lo
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// 8 codes times 2^(byte - 127) in bf16
+// 8 codes times 2^(byte - 127) in bf16; a NaN scale makes NaN codes of all of them
 __device__ __forceinline__ bf16x8 to_bf16(int c0, int c1, unsigned byte) {
-    if (byte == 255) {
-        const __bf16 nan = __builtin_bit_cast(__bf16, (unsigned short)0x7fc0);
-        return bf16x8{nan, nan, nan, nan, nan, nan, nan, nan};
-    }
-    const float scale = scale_value(byte);
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)c0, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)c0, scale, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)c1, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)c1, scale, true);
+    const unsigned poison = byte == 255 ? 0x7f7f7f7fu : 0u;
+    const float scale = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x3f800000u : byte << 23);
+    const unsigned d0 = (unsigned)c0 | poison, d1 = (unsigned)c1 | poison;
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d0, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d0, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d1, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d1, scale, true);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -388,7 +386,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
 
     // ---- epilogue: this wave's rows of c through LDS (the ring and the scales are done with), then whole rows with 16-byte stores.
     // PASS matrix tiles along m at a time, as many as fit; a tile inside c takes straight-line code, eight stores in flight.
+    // The lane's number is asked for anew: nothing that depends on it stays in registers through the steps.
     __syncthreads();
+    const int el = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), em = el & 31, eh = el >> 5;
     constexpr int ES = (int)sizeof(T), ROWB = 32 * NI * ES, PITCH = ROWB + 16, PIECES = ROWB / 16, EV = 16 / ES;
     constexpr int PASS = NJ * 4 * 32 * PITCH <= RING + ROWS * G8_SPITCH ? NJ : NJ / 2;
     static_assert(BN <= 256 && PASS * 4 * 32 * PITCH <= RING + ROWS * G8_SPITCH, "epilogue scratch");
@@ -403,19 +403,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int col = i * 32 + 8 * g + 4 * hh;
+                const int col = i * 32 + 8 * g + 4 * eh;
                 const f32x4 b4 = *(const f32x4*)(bias + wn * 32 * NI + col);
 #pragma unroll
                 for (int j = 0; j < PASS; ++j) {
                     t4 v;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j0 + j][4 * g + e] + b4[e]);
-                    *(t4*)(scr + (j * 32 + ml) * PITCH + col * ES) = v;
+                    *(t4*)(scr + (j * 32 + em) * PITCH + col * ES) = v;
                 }
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wave's own scratch: no barrier)
         constexpr int UNITS = PASS * 32 * PIECES / 64, STEP = 64 / PIECES;   // a unit: STEP rows
-        const int r = lane / PIECES, c = lane % PIECES;
+        const int r = el / PIECES, c = el % PIECES;
         const char* const from = scr + r * PITCH + c * 16;
         if (inside) {
             T* out = (T*)p.c + (row0 + j0 * 32 + r) * p.ldc + col0 + c * EV;
