@@ -440,7 +440,10 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
  * for have to lie in fp32's normal range (smaller ones count as 0). */
 int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
                   const uint8_t* b_scale_dev, int64_t ldsb, int b_tile, const void* bias_dev, int bias_dtype, void* c_dev, int c_dtype,
-                  int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream);
+                  int64_t ldc, int64_t m, int64_t n, int64_t k, void* work_dev, int64_t work_bytes, void* stream);
+/* Bytes of workspace with which ml_fp8_matmul may cut a long k over workgroups (few tiles; 0: it would not): fp32 parts, joined in order.
+ * Without it (NULL, fewer bytes, or not on 16 bytes) the product is computed uncut. */
+int64_t ml_fp8_matmul_work(int64_t m, int64_t n, int64_t k, int c_dtype);
 /* A linear layer with both operands in 8 bits, forward and backward, each in one call: y (m, n) = Q(x) . Q(w)^T [+ bias], x (m, k) in 1 x 128
  * blocks, w (n, k) in tiles, y of x's type; dx = Q(dy) . Q(w); dw = Q(dy^T) . Q(x^T)^T, 1 x 128 blocks along the batch; db = column sums of
  * dy.  bytes3 = {forward's workspace, what backward needs (kept by the caller between the two calls), backward's workspace}, all aligned to

@@ -125,7 +125,8 @@ SIGNATURES = {
     'ml_matching_last_error': (c_char_p, []),
     'ml_fp8_quantize': (c_int, [_P, c_int, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P]),
     'ml_fp8_matmul': (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int64, _P, c_int64, c_int, _P, c_int, _P, c_int, c_int64, c_int64,
-                              c_int64, c_int64, _P]),
+                              c_int64, c_int64, _P, c_int64, _P]),
+    'ml_fp8_matmul_work': (c_int64, [c_int64, c_int64, c_int64, c_int]),
     'ml_fp8_linear_sizes': (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_int, _P]),
     'ml_fp8_linear': (c_int, [_P, c_int, c_int64, _P, c_int, c_int64, _P, c_int, _P, c_int64, c_int64, c_int64, c_int64, c_int, c_int, _P,
                               _P, _P]),

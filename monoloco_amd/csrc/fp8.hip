@@ -1,6 +1,8 @@
 // fp8.hip -- C entry points of the 8-bit residual-block operators: quantisation into e4m3 blocks of 128, the block-scaled product,
 // root-mean-square norm with residual (8-bit or plain output) and its backward pass.  All are asynchronous on the caller's stream,
 // allocate nothing and keep nothing between calls (a workspace is an argument), so they may be captured into a graph.
+#include <algorithm>
+
 #include "fp8_gemm.h"
 #include "fp8_quant.h"
 #include "norm_kernels.h"
@@ -58,12 +60,51 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
 //     against 24.6 with 128 x 128, 32768 x 1024 x 1024 44.7 against 48.9; 2048 x 4096 x 4096 (128) 47.1 against 40.9, 4096^3 (256) 59.7
 //     against 77.9; below k = 1024 a tile's start and end outweigh its steps.  fp32: 2560 x 4096 x 4096 (160) 97 against 98, 4096^3 114 against
 //     133, 8192^3 856 against 986.
+//   Few tiles and a long k (the weight gradient of a large batch): 128 x 128 tiles whose blocks of k are shared by several workgroups, where
+//     that is estimated to be faster: gemm_splits.
+struct Tiles {
+    long t256, t128, t64;
+    Tiles(long m, long n) {
+        auto across = [&](long t) { return (m + t - 1) / t * ((n + t - 1) / t); };
+        t256 = across(256), t128 = across(128), t64 = across(64);
+    }
+};
+
+// In how many parts k is cut, 1: not at all.  Estimates in us, from products of 256 .. 2048 rows and columns and k = 4096 .. 65536: a step of 64
+// takes a 128 x 128 tile 0.29 (fp32 results: 0.55) alone on its CU and 0.55 (0.95) beside another one, a lone 64 x 64 tile 0.17 (0.29); the
+// parts are written and read at 4.5 TB/s and joined by a launch of 4.  Cut where that says 18 % less, into the parts with the least.
+// Uncut against cut, bf16 (fp32): 1024 x 1024 x 65536 171 against 86 (292, 149), x 16384 44 against 32 (75, 51); 1024 x 2048 x 8192 36.5
+// against 32.0 (left: 65, 58); 256 x 256 x 65536 156 against 23 (287, 27); 512 x 512 x 8192 19.7 against 15.9 (38, 21); 128 x 4096 x 16384 41
+// against 24 (75, 34); fp32 1920 x 1920 x 16384 195 against 141.  Left uncut in bf16: 256 x 256 x 4096 11.1 against 11.2, 1920 x 1920 x 16384 73
+// against 92 in two parts.
+int gemm_splits(long m, long n, long k, bool half) {
+    const Tiles t(m, n);
+    const long kb = (k + QB - 1) / QB;
+    if (m <= 64 || t.t128 >= 256 || kb < 16) return 1;
+    const double steps = 2.0 * kb, lone = half ? 0.29 : 0.55, pair = half ? 0.55 : 0.95;
+    const double uncut = half ? (t.t64 <= 256 ? 0.17 : 0.29) : 0.29 * std::max(1.0, 0.75 * t.t64 / 256);
+    const long most = std::min({512 / t.t128, kb / 8, 64L});
+    int best = 1;
+    double least = 0.82 * steps * uncut;
+    for (long s = 2; s <= most; ++s) {
+        const double us = steps / s * (s * t.t128 <= 256 ? lone : pair) + s * (double)(m * n) * 8.0 / 4.5e6 + 4.0;
+        if (us < least) least = us, best = (int)s;
+    }
+    return best;
+}
+
+int64_t gemm_work_bytes(long m, long n, long k, bool half) {
+    const int s = gemm_splits(m, n, k, half);
+    return s > 1 ? (int64_t)s * m * n * 4 : 0;
+}
+
 template <typename T>
-void launch_gemm(const GemmParams& p, hipStream_t s) {
+void launch_gemm(const GemmParams& p, float* work, int64_t work_bytes, hipStream_t s) {
     constexpr bool HALF = sizeof(T) == 2;
     const bool ring = p.fast_a && p.fast_b && p.lda < (1L << 23) && p.ldb < (1L << 23);
-    auto across = [&](long t) { return (p.m + t - 1) / t * ((p.n + t - 1) / t); };
-    const long t256 = across(256), t128 = across(128), t64 = across(64);
+    const Tiles t(p.m, p.n);
+    const long t256 = t.t256, t128 = t.t128, t64 = t.t64;
+    const int splits = ring && work && (uintptr_t)work % 16 == 0 && work_bytes >= gemm_work_bytes(p.m, p.n, p.k, HALF) ? gemm_splits(p.m, p.n, p.k, HALF) : 1;
     auto tiles = [](long size, int t) { return (int)((size + t - 1) / t); };
     const long g16 = (p.n + 15) / 16;
     if (p.m <= 16 && fits(g16, 512)) {
@@ -74,6 +115,11 @@ void launch_gemm(const GemmParams& p, hipStream_t s) {
         if constexpr (!HALF) fp8_gemm_rows_kernel<T, 4, 2><<<(unsigned)g16, 512, 0, s>>>(p);
     } else if (!ring) {
         fp8_gemm64_kernel<T><<<(unsigned)t64, 256, 0, s>>>(p);
+    } else if (splits > 1) {
+        GemmParams q = p;
+        q.c = work;
+        fp8_gemm_ring_kernel<T, 2, 2, true><<<dim3((unsigned)t128, (unsigned)splits), 256, 0, s>>>(q, tiles(p.m, 128), tiles(p.n, 128));
+        join_splits_kernel<T><<<(unsigned)((p.m * p.n + 1023) / 1024), 256, 0, s>>>(p, work, splits);
     } else if (p.k >= 1024 && (t256 > 256 || (t256 >= 160 && p.k >= 2048))) {
         bool streamed = false;
         if constexpr (HALF) {
@@ -142,9 +188,13 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
     return ops_launched("ml_fp8_quantize");
 }
 
+int64_t ml_fp8_matmul_work(int64_t m, int64_t n, int64_t k, int c_dtype) {
+    return m <= 0 || n <= 0 || k <= 0 || m > (1LL << 33) || n > (1LL << 33) ? 0 : gemm_work_bytes(m, n, k, c_dtype != ML_F32);
+}
+
 int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
                   const uint8_t* b_scale_dev, int64_t ldsb, int b_tile, const void* bias_dev, int bias_dtype, void* c_dev, int c_dtype,
-                  int64_t ldc, int64_t m, int64_t n, int64_t k, void* stream) {
+                  int64_t ldc, int64_t m, int64_t n, int64_t k, void* work_dev, int64_t work_bytes, void* stream) {
     const int es = elem_size(c_dtype);
     if (!es || (bias_dev && !elem_size(bias_dtype)) || m < 0 || n < 0 || k < 0) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: bad type %d, %d or size", c_dtype, bias_dtype);
     if (m == 0 || n == 0) return ML_OK;
@@ -157,7 +207,7 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
                  (long)m, (long)n, (long)k, (long)ldc, 0, 0};
     p.fast_a = rows_aligned(a_dev, lda, 1, 16), p.fast_b = rows_aligned(b_dev, ldb, 1, 16);
     const hipStream_t s = (hipStream_t)stream;
-    with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, s); });
+    with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, (float*)work_dev, work_bytes, s); });
     return ops_launched("ml_fp8_matmul");
 }
 
@@ -167,22 +217,26 @@ static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; 
 namespace {
 struct LinearPlan {
     int64_t kb, nb, mb, ldk, ldn, ldm;                  // blocks; row strides of codes along k, n, m
-    int64_t qx, sx, qw, sw, forward;                    // forward's workspace
+    int64_t qx, sx, qw, sw, fsplit, forward;            // forward's workspace (fsplit, bsplit: parts of a product whose k is cut)
     int64_t qxt, sxt, qwt, swt, saved;                  // what the backward pass needs
-    int64_t qd, sd, qdt, sdt, part, backward;           // backward's workspace
+    int64_t qd, sd, qdt, sdt, part, bsplit, backward;   // backward's workspace
     LinearPlan(int64_t m, int64_t n, int64_t k, bool need_dx, bool need_dw, bool need_db) {
         kb = (k + QB - 1) / QB, nb = (n + QB - 1) / QB, mb = (m + QB - 1) / QB;
         ldk = round_up(k, 16), ldn = round_up(n, 16), ldm = round_up(m, 16);
+        auto most = [](int64_t a, int64_t b, int64_t c) { return std::max(ml_fp8_matmul_work(a, b, c, ML_BF16), ml_fp8_matmul_work(a, b, c, ML_F32)); };
         int64_t at = 0;
         auto take = [&](int64_t bytes) { const int64_t r = at; at += round_up(bytes, 256); return r; };
-        qx = take(m * ldk), sx = take(m * kb), qw = take(n * ldk), sw = take(nb * kb), forward = at;
+        qx = take(m * ldk), sx = take(m * kb), qw = take(n * ldk), sw = take(nb * kb);
+        fsplit = take(most(m, n, k)), forward = at;
         at = 0;
         qxt = take(need_dw ? k * ldm : 0), sxt = take(need_dw ? k * mb : 0);
         qwt = take(need_dx ? k * ldn : 0), swt = take(need_dx ? kb * nb : 0), saved = at;
         at = 0;
         qd = take(need_dx ? m * ldn : 0), sd = take(need_dx ? m * nb : 0);
         qdt = take(need_dw ? n * ldm : 0), sdt = take(need_dw ? n * mb : 0);
-        part = take(need_db ? mb * n * 4 : 0), backward = at;
+        part = take(need_db ? mb * n * 4 : 0);
+        const int64_t dx = need_dx ? most(m, k, n) : 0, dw = need_dw ? most(n, k, m) : 0;   // (one after the other)
+        bsplit = take(dx > dw ? dx : dw), backward = at;
     }
 };
 }  // namespace
@@ -205,7 +259,8 @@ int ml_fp8_linear(const void* x_dev, int x_dtype, int64_t ldx, const void* w_dev
     if (!rc)
         rc = ml_fp8_quantize(w_dev, w_dtype, n, k, ldw, 1, wk + l.qw, l.ldk, wk + l.sw, l.kb, need_dx ? sv + l.qwt : nullptr, l.ldn, need_dx ? sv + l.swt : nullptr,
                              l.nb, nullptr, stream);
-    if (!rc) rc = ml_fp8_matmul(wk + l.qx, l.ldk, wk + l.sx, l.kb, 0, wk + l.qw, l.ldk, wk + l.sw, l.kb, 1, bias_dev, bias_dtype, y_dev, x_dtype, ldy, m, n, k, stream);
+    if (!rc) rc = ml_fp8_matmul(wk + l.qx, l.ldk, wk + l.sx, l.kb, 0, wk + l.qw, l.ldk, wk + l.sw, l.kb, 1, bias_dev, bias_dtype, y_dev, x_dtype, ldy, m, n, k, wk + l.fsplit,
+                              l.forward - l.fsplit, stream);
     return rc;
 }
 
@@ -224,8 +279,10 @@ int ml_fp8_linear_backward(const void* dy_dev, int dy_dtype, int64_t ldy, const 
                              dw ? wk + l.sdt : nullptr, l.mb, db_dev ? (float*)(wk + l.part) : nullptr, stream);
     else if (db_dev)
         rc = column_sums(dy_dev, dy_dtype, m, n, ldy, (float*)(wk + l.part), (hipStream_t)stream);
-    if (!rc && dx) rc = ml_fp8_matmul(wk + l.qd, l.ldn, wk + l.sd, l.nb, 0, sv + l.qwt, l.ldn, sv + l.swt, l.nb, 1, nullptr, 0, dx_dev, dx_dtype, k, m, k, n, stream);
-    if (!rc && dw) rc = ml_fp8_matmul(wk + l.qdt, l.ldm, wk + l.sdt, l.mb, 0, sv + l.qxt, l.ldm, sv + l.sxt, l.mb, 0, nullptr, 0, dw_dev, dw_dtype, k, n, k, m, stream);
+    if (!rc && dx) rc = ml_fp8_matmul(wk + l.qd, l.ldn, wk + l.sd, l.nb, 0, sv + l.qwt, l.ldn, sv + l.swt, l.nb, 1, nullptr, 0, dx_dev, dx_dtype, k, m, k, n, wk + l.bsplit, l.backward - l.bsplit,
+                                     stream);
+    if (!rc && dw) rc = ml_fp8_matmul(wk + l.qdt, l.ldm, wk + l.sdt, l.mb, 0, sv + l.qxt, l.ldm, sv + l.sxt, l.mb, 0, nullptr, 0, dw_dev, dw_dtype, k, n, k, m, wk + l.bsplit, l.backward - l.bsplit,
+                                     stream);
     if (!rc && db_dev) rc = ml_sum_rows((const float*)(wk + l.part), m ? l.mb : 0, n, db_dev, db_dtype, stream);
     return rc;
 }

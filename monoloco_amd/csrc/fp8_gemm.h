@@ -157,8 +157,11 @@ constexpr int G8_CHUNK = 32;              // blocks of 128 whose scales are in L
 constexpr int G8_REQ0 = 8;               // streaming kernel: the product of a step behind which its requests begin
 constexpr int G8_SPITCH = G8_CHUNK + 4;   // bytes per row of them: 32 rows fall into different banks
 
-template <typename T, int NI, int NJ>
+// SPLIT: gridDim.y workgroups share the blocks of k of one tile; each stores its part of the sum in fp32 (part y at c + y m n floats, no bias),
+// join_splits_kernel adds them in order.
+template <typename T, int NI, int NJ, bool SPLIT = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 16 ? 1 : NI * NJ == 4 ? 2 : 4))) void fp8_gemm_ring_kernel(GemmParams p, int mt, int nt) {
+    using OT = std::conditional_t<SPLIT, float, T>;   // what is stored
     constexpr int BN = 64 * NI, BM = 64 * NJ, ROWS = BN + BM, SLOT = ROWS * 64, RING = 4 * SLOT, NQ = NI + NJ;
     __shared__ __attribute__((aligned(16))) char smem[RING + ROWS * G8_SPITCH + BN * 4];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wn = w & 1, wm = w >> 1;
@@ -171,6 +174,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
     const int grp = tile / (4 * nt), rem = tile - grp * 4 * nt, gm = min(4, mt - grp * 4);
     const long m0 = (long)(grp * 4 + rem % gm) * BM, n0 = (long)(rem / gm) * BN;
 
+    if constexpr (SPLIT) {   // this workgroup's blocks of k (the last one's may end in a partial block)
+        const long kb = (p.k + QB - 1) / QB, each = (kb + gridDim.y - 1) / gridDim.y, b0 = min(each * blockIdx.y, kb), b1 = min(b0 + each, kb);
+        p.a += b0 * QB, p.b += b0 * QB, p.sa += b0, p.sb += b0;
+        p.k = min(b1 * QB, p.k) - min(b0 * QB, p.k);
+        p.c = (float*)p.c + blockIdx.y * p.m * p.n;
+        p.ldc = p.n;
+        p.bias = nullptr;
+    }
     const int nkb = (int)(p.k / QB);                  // whole blocks of 128
     const int nst = 2 * nkb;                          // steps of 64 in the ring
     // ---- DMA: instruction q of this wave fetches 16 rows x 64 bytes; lane = row * 4 + piece, LDS linear, bank swizzle on the source
@@ -389,12 +400,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
     // The lane's number is asked for anew: nothing that depends on it stays in registers through the steps.
     __syncthreads();
     const int el = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), em = el & 31, eh = el >> 5;
-    constexpr int ES = (int)sizeof(T), ROWB = 32 * NI * ES, PITCH = ROWB + 16, PIECES = ROWB / 16, EV = 16 / ES;
+    constexpr int ES = (int)sizeof(OT), ROWB = 32 * NI * ES, PITCH = ROWB + 16, PIECES = ROWB / 16, EV = 16 / ES;
     constexpr int PASS = NJ * 4 * 32 * PITCH <= RING + ROWS * G8_SPITCH ? NJ : NJ / 2;
     static_assert(BN <= 256 && PASS * 4 * 32 * PITCH <= RING + ROWS * G8_SPITCH, "epilogue scratch");
     char* const scr = smem + w * PASS * 32 * PITCH;
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    typedef T tv __attribute__((ext_vector_type(EV)));
+    typedef OT t4 __attribute__((ext_vector_type(4)));
+    typedef OT tv __attribute__((ext_vector_type(EV)));
     const bool inside = m0 + BM <= p.m && n0 + BN <= p.n;
     const long row0 = m0 + wm * 32 * NJ, col0 = n0 + wn * 32 * NI;
 #pragma unroll
@@ -409,7 +420,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
                 for (int j = 0; j < PASS; ++j) {
                     t4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j0 + j][4 * g + e] + b4[e]);
+                    for (int e = 0; e < 4; ++e) v[e] = (OT)(acc[i][j0 + j][4 * g + e] + b4[e]);
                     *(t4*)(scr + (j * 32 + em) * PITCH + col * ES) = v;
                 }
             }
@@ -418,7 +429,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
         const int r = el / PIECES, c = el % PIECES;
         const char* const from = scr + r * PITCH + c * 16;
         if (inside) {
-            T* out = (T*)p.c + (row0 + j0 * 32 + r) * p.ldc + col0 + c * EV;
+            OT* out = (OT*)p.c + (row0 + j0 * 32 + r) * p.ldc + col0 + c * EV;
             const long by = (long)STEP * p.ldc;
 #pragma unroll
             for (int u = 0; u < UNITS; u += 8) {
@@ -440,7 +451,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
                 const long row = row0 + j0 * 32 + r + u * STEP;
                 const tv v = *(const tv*)(from + u * STEP * PITCH);
                 if (row < p.m && col < p.n) {
-                    T* const out = (T*)p.c + row * p.ldc + col;
+                    OT* const out = (OT*)p.c + row * p.ldc + col;
                     if (col + EV <= p.n) {
                         store_any(out, v);
                     } else {
@@ -452,6 +463,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NI * NJ == 
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// c = the sum of the parts, in order, + bias; a part is (m, n) without gaps
+template <typename T>
+__global__ __launch_bounds__(256) void join_splits_kernel(GemmParams p, const float* __restrict__ part, int splits) {
+    const long mn = p.m * p.n, i0 = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i0 >= mn) return;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (i0 + 4 <= mn) {
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) v += load_any<f32x4>(part + s * mn + i0);
+    } else {
+        for (int s = 0; s < splits; ++s)
+            for (int e = 0; e < 4; ++e)
+                if (i0 + e < mn) v[e] += part[s * mn + i0 + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const long i = i0 + e, row = i / p.n, col = i - row * p.n;
+        if (i < mn) ((T*)p.c)[row * p.ldc + col] = (T)(v[e] + bias_at(p, col));
     }
 }
 

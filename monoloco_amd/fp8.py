@@ -136,6 +136,11 @@ def _scales_of(name, codes, scale):
                      % (name, tuple(shape), scale.dtype, (rows, k), SCALES, rows, kb, -(-rows // BLOCK), kb))
 
 
+@functools.lru_cache(maxsize=1024)
+def _matmul_work(m, n, k, dtype):
+    return int(_lib.load().ml_fp8_matmul_work(m, n, k, dtype))
+
+
 def matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16, out=None):
     """a (m, k) . b (n, k)^T [+ bias (n)] of e4m3 codes with their block scales -> (m, n) in ``out_dtype`` (fp32, bf16, fp16), accumulated
     in fp32 and rounded once.  16-bit results come from the 8-bit matrix instructions (1.5e-5 of the result's norm beside the rounding), fp32
@@ -168,8 +173,12 @@ def matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16, out=None
         _need(not (out.requires_grad and torch.is_grad_enabled()), "matmul is not differentiable: out must not require a gradient")
     if m and n:
         a, b, a_scale, b_scale = _rows(a), _rows(b), _rows(a_scale), _rows(b_scale)
+        dt = DTYPES[out.dtype]
+        size = _matmul_work(m, n, k, dt)
+        work = torch.empty((size,), dtype=torch.uint8, device=a.device) if size else None
         _run(index, _lib.load().ml_fp8_matmul, a.data_ptr(), _ld(a), a_scale.data_ptr(), _ld(a_scale), a_tile, b.data_ptr(), _ld(b), b_scale.data_ptr(), _ld(b_scale),
-             b_tile, bias.data_ptr() if bias is not None else None, DTYPES[bias.dtype] if bias is not None else 0, out.data_ptr(), DTYPES[out.dtype], _ld(out), m, n, k)
+             b_tile, bias.data_ptr() if bias is not None else None, DTYPES[bias.dtype] if bias is not None else 0, out.data_ptr(), dt, _ld(out), m, n, k,
+             work.data_ptr() if size else None, size)
     if given:
         torch.autograd.graph.increment_version(out)
     return out

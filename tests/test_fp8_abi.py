@@ -32,14 +32,26 @@ def test_quantize_refusals(hip_lib):
 
 def test_matmul_refusals(hip_lib):
     f = hip_lib.ml_fp8_matmul
-    _refused(hip_lib, 1, 'bad type', f, P, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, P, 9, 4, 4, 4, 16, None)
-    _refused(hip_lib, 1, 'bad type', f, P, 16, P, 1, 0, P, 16, P, 1, 0, P, 5, P, 0, 4, 4, 4, 16, None)
-    _refused(hip_lib, 1, 'null pointer', f, None, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, P, 0, 4, 4, 4, 16, None)
-    _refused(hip_lib, 1, 'null pointer', f, P, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, None, 0, 4, 4, 4, 16, None)
+    _refused(hip_lib, 1, 'bad type', f, P, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, P, 9, 4, 4, 4, 16, None, 0, None)
+    _refused(hip_lib, 1, 'bad type', f, P, 16, P, 1, 0, P, 16, P, 1, 0, P, 5, P, 0, 4, 4, 4, 16, None, 0, None)
+    _refused(hip_lib, 1, 'null pointer', f, None, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, P, 0, 4, 4, 4, 16, None, 0, None)
+    _refused(hip_lib, 1, 'null pointer', f, P, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, None, 0, 4, 4, 4, 16, None, 0, None)
     for lda, ldsa, ldb, ldsb, ldc in ((129, 2, 130, 2, 4), (130, 1, 130, 2, 4), (130, 2, 129, 2, 4), (130, 2, 130, 1, 4), (130, 2, 130, 2, 3)):
-        _refused(hip_lib, 1, 'row stride', f, P, lda, P, ldsa, 0, P, ldb, P, ldsb, 0, None, 0, P, 0, ldc, 4, 4, 130, None)
-    _refused(hip_lib, 4, 'too large', f, P, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, P, 0, 1 << 30, 1 << 30, 1 << 30, 16, None)
-    assert f(None, 16, None, 1, 0, None, 16, None, 1, 0, None, 0, None, 0, 4, 0, 4, 16, None) == 0
+        _refused(hip_lib, 1, 'row stride', f, P, lda, P, ldsa, 0, P, ldb, P, ldsb, 0, None, 0, P, 0, ldc, 4, 4, 130, None, 0, None)
+    _refused(hip_lib, 4, 'too large', f, P, 16, P, 1, 0, P, 16, P, 1, 0, None, 0, P, 0, 1 << 30, 1 << 30, 1 << 30, 16, None, 0, None)
+    assert f(None, 16, None, 1, 0, None, 16, None, 1, 0, None, 0, None, 0, 4, 0, 4, 16, None, 0, None) == 0
+
+
+def test_matmul_workspace(hip_lib):
+    """Only few tiles with a long k are cut, and the parts stay far below what the operands of such a product take."""
+    work = hip_lib.ml_fp8_matmul_work
+    assert work(0, 5, 5, 0) == work(5, 0, 5, 0) == work(5, 5, 0, 0) == 0
+    for m, n, k in ((1, 4096, 4096), (512, 1024, 1024), (65536, 1024, 1024), (8192, 8192, 8192), (4096, 4096, 16384)):
+        assert work(m, n, k, 1) == 0 and work(m, n, k, 0) == 0
+    for m, n, k in ((1024, 1024, 65536), (145, 568, 17801), (256, 256, 100000)):
+        for dt in (0, 1, 2):
+            parts, rest = divmod(work(m, n, k, dt), m * n * 4)
+            assert rest == 0 and 2 <= parts <= 64 and parts <= k // 1024, (m, n, k, dt, parts)
 
 
 def test_norm_refusals(hip_lib):

@@ -155,7 +155,7 @@ def check_product(c, a, sa, at, b, sb, bt, bias, dtype):
 
 PRODUCTS = [(1, 1, 1), (1, 9, 34), (1, 1024, 1024), (2, 16, 128), (7, 100, 1111), (16, 256, 256), (17, 129, 260), (33, 1000, 4096), (64, 64, 64),
             (65, 63, 129), (100, 300, 127), (128, 256, 384), (129, 257, 2048), (200, 512, 1000), (256, 256, 128), (257, 513, 640), (331, 1000, 1111),
-            (512, 1024, 1024), (700, 70, 16), (1025, 1281, 144)]
+            (512, 1024, 1024), (700, 70, 16), (1025, 1281, 144), (66, 100, 20000), (145, 201, 17801), (300, 260, 8192), (512, 512, 4100)]
 
 
 @pytest.mark.parametrize('m,n,k', PRODUCTS)
@@ -221,6 +221,50 @@ def test_matmul_many_tiles(cuda_device, m, n, k, bias, dtype):
     assert torch.equal(fp8.matmul(wa, sa.view(E8), wb, sb.view(E8), bias=bv, out=big[1:-1, 3:3 + n]), c)
     big[1:-1, 3:3 + n] = 7.0
     assert bool((big == 7.0).all())
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,n,k', [(145, 201, 17801), (130, 260, 8192)])
+def test_matmul_cut(cuda_device, hip_lib, m, n, k, dtype):
+    """Few tiles and a long k, shared by several workgroups: a strided output at an odd address with nothing around it written, the same
+    bits on two streams at once and in a replayed graph, the uncut product without a workspace."""
+    assert hip_lib.ml_fp8_matmul_work(m, n, k, fp8.DTYPES[dtype]) > 0
+    a, sa, b, sb = operands(m + n, m, n, k, False, False)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(1))
+    dev, bv = [t.to(cuda_device) for t in (a, sa, b, sb)], bias.to(cuda_device)
+    wide = [torch.zeros((t.shape[0], k + -k % 16), dtype=torch.uint8, device=cuda_device) for t in (a, b)]
+    for t, v in zip(wide, (dev[0], dev[2])):
+        t[:, :k] = v.view(torch.uint8)
+    args = [wide[0][:, :k].view(F8), dev[1], wide[1][:, :k].view(F8), dev[3]]
+    c = fp8.matmul(*args, bias=bv, out_dtype=dtype)
+    check_product(c, a, sa, False, b, sb, False, bias, dtype)
+    big = torch.full((m + 2, n + 5), 7.0, dtype=dtype, device=cuda_device)
+    assert torch.equal(fp8.matmul(*args, bias=bv, out=big[1:-1, 3:3 + n]), c)
+    big[1:-1, 3:3 + n] = 7.0
+    assert bool((big == 7.0).all())
+    torch.cuda.synchronize()
+    side, out = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for i, st in enumerate(side):
+        with torch.cuda.stream(st):
+            for _ in range(5):
+                out[i] = fp8.matmul(*args, bias=bv, out_dtype=dtype)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], c) and torch.equal(out[1], c)
+    graph, into = torch.cuda.CUDAGraph(), torch.zeros_like(c)
+    with torch.cuda.graph(graph):
+        fp8.matmul(*args, bias=bv, out=into)
+    for _ in range(3):
+        into.zero_()
+        graph.replay()
+        assert torch.equal(fp8.matmul(*args, bias=bv, out_dtype=dtype), c)
+        torch.cuda.synchronize()
+        assert torch.equal(into, c)
+    plain = torch.empty_like(c)
+    x, w = args[0], args[2]
+    assert hip_lib.ml_fp8_matmul(x.data_ptr(), x.stride(0), dev[1].data_ptr(), dev[1].stride(0), 0, w.data_ptr(), w.stride(0), dev[3].data_ptr(),
+                                 dev[3].stride(0), 0, bv.data_ptr(), fp8.DTYPES[bv.dtype], plain.data_ptr(), fp8.DTYPES[dtype], n, m, n, k, None, 0,
+                                 torch.cuda.current_stream().cuda_stream) == 0
+    check_product(plain, a, sa, False, b, sb, False, bias, dtype)
 
 
 def test_matmul_views_pads_and_out(cuda_device):
@@ -310,6 +354,12 @@ def test_linear(cuda_device, m, n, k, dtype):
         args = [t.detach().clone().requires_grad_(i == leaf) for i, t in enumerate((xs, ws, bs))]
         got, = torch.autograd.grad(fp8.linear(*args), [args[leaf]], dy.to(cuda_device))
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_linear_many_rows(cuda_device, dtype):
+    """The weight gradient sums over the rows: a long k with few tiles, shared by several workgroups."""
+    test_linear(cuda_device, 9001, 130, 200, dtype)
 
 
 def test_linear_mixed_types(cuda_device):
