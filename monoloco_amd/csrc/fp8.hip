@@ -61,7 +61,7 @@ void launch_norm_back(const NormBackParams& p, unsigned g, hipStream_t s) {
 //     against 77.9; below k = 1024 a tile's start and end outweigh its steps.  fp32: 2560 x 4096 x 4096 (160) 97 against 98, 4096^3 114 against
 //     133, 8192^3 856 against 986.
 //   Few tiles and a long k (the weight gradient of a large batch): 128 x 128 tiles whose blocks of k are shared by several workgroups, where
-//     that is estimated to be faster: gemm_splits.
+//     that is estimated to be faster than the kernels above: gemm_splits.
 struct Tiles {
     long t256, t128, t64;
     Tiles(long m, long n) {
@@ -70,24 +70,26 @@ struct Tiles {
     }
 };
 
-// In how many parts k is cut, 1: not at all.  Estimates in us, from products of 256 .. 2048 rows and columns and k = 4096 .. 65536: a step of 64
-// takes a 128 x 128 tile 0.29 (fp32 results: 0.55) alone on its CU and 0.55 (0.95) beside another one, a lone 64 x 64 tile 0.17 (0.29); the
-// parts are written and read at 4.5 TB/s and joined by a launch of 4.  Cut where that says 18 % less, into the parts with the least.
-// Uncut against cut, bf16 (fp32): 1024 x 1024 x 65536 171 against 86 (292, 149), x 16384 44 against 32 (75, 51); 1024 x 2048 x 8192 36.5
-// against 32.0 (left: 65, 58); 256 x 256 x 65536 156 against 23 (287, 27); 512 x 512 x 8192 19.7 against 15.9 (38, 21); 128 x 4096 x 16384 41
-// against 24 (75, 34); fp32 1920 x 1920 x 16384 195 against 141.  Left uncut in bf16: 256 x 256 x 4096 11.1 against 11.2, 1920 x 1920 x 16384 73
-// against 92 in two parts.
+// In how many parts k is cut, 1: not at all.  Estimates in us, from products of 9 .. 2048 rows and k = 4096 .. 65536: a step of 64 takes a
+// 128 x 128 tile 0.29 (fp32 results: 0.55) alone on its CU and 0.55 (0.95) beside another one, a lone 64 x 64 tile 0.17 (0.29), the kernels of
+// few rows 0.068 (m <= 16), 0.11 (m <= 32) and 0.2 (fp32, m <= 64); the operands come at 5.2 TB/s at best, the parts are written and read at
+// 4.5 and joined by a launch of 4. Cut where that says 18 % less, into the parts with the least.  Uncut against cut, bf16 (fp32): 1024 x 1024 x
+// 65536 171 against 86 (292, 149), x 16384 44 against 32 (75, 51); 1024 x 2048 x 8192 36.5 against 32.0 (left: 65, 58); 256 x 256 x 65536 156
+// against 23 (287, 27); 512 x 512 x 8192 19.7 against 15.9 (38, 21); 128 x 4096 x 16384 41 against 24 (75, 34); 9 x 1024 x 65536 72 against 21
+// (74, 31), x 16384 19.9 against 13.0 (20.9, 18.5); 32 x 1024 x 8192 18.6 against 12.3 (left: 19.0, 17.5); fp32 1920 x 1920 x 16384 195 against
+// 141.  Left uncut in bf16: 9 x 1024 x 8192 10.9 against 11.5, 1 x 4096 x 16384 17.8 against 18.8, 256 x 256 x 4096 11.1 against 11.2, 1920 x
+// 1920 x 16384 73 against 92 in two parts.
 int gemm_splits(long m, long n, long k, bool half) {
     const Tiles t(m, n);
     const long kb = (k + QB - 1) / QB;
-    if (m <= 64 || t.t128 >= 256 || kb < 16) return 1;
-    const double steps = 2.0 * kb, lone = half ? 0.29 : 0.55, pair = half ? 0.55 : 0.95;
-    const double uncut = half ? (t.t64 <= 256 ? 0.17 : 0.29) : 0.29 * std::max(1.0, 0.75 * t.t64 / 256);
+    if (t.t128 >= 256 || kb < 16) return 1;
+    const double steps = 2.0 * kb, bytes = (double)(m + n) * k, lone = half ? 0.29 : 0.55, pair = half ? 0.55 : 0.95;
+    const double uncut = m <= 16 ? 0.068 : m <= 32 ? 0.11 : half ? (t.t64 <= 256 ? 0.17 : 0.29) : m <= 64 ? 0.2 : 0.29 * std::max(1.0, 0.75 * t.t64 / 256);
     const long most = std::min({512 / t.t128, kb / 8, 64L});
     int best = 1;
     double least = 0.82 * steps * uncut;
     for (long s = 2; s <= most; ++s) {
-        const double us = steps / s * (s * t.t128 <= 256 ? lone : pair) + s * (double)(m * n) * 8.0 / 4.5e6 + 4.0;
+        const double us = std::max(steps / s * (s * t.t128 <= 256 ? lone : pair), bytes / 5.2e6) + s * (double)(m * n) * 8.0 / 4.5e6 + 4.0;
         if (us < least) least = us, best = (int)s;
     }
     return best;
@@ -107,7 +109,12 @@ void launch_gemm(const GemmParams& p, float* work, int64_t work_bytes, hipStream
     const int splits = ring && work && (uintptr_t)work % 16 == 0 && work_bytes >= gemm_work_bytes(p.m, p.n, p.k, HALF) ? gemm_splits(p.m, p.n, p.k, HALF) : 1;
     auto tiles = [](long size, int t) { return (int)((size + t - 1) / t); };
     const long g16 = (p.n + 15) / 16;
-    if (p.m <= 16 && fits(g16, 512)) {
+    if (splits > 1) {
+        GemmParams q = p;
+        q.c = work;
+        fp8_gemm_ring_kernel<T, 2, 2, true><<<dim3((unsigned)t128, (unsigned)splits), 256, 0, s>>>(q, tiles(p.m, 128), tiles(p.n, 128));
+        join_splits_kernel<T><<<(unsigned)((p.m * p.n + 1023) / 1024), 256, 0, s>>>(p, work, splits);
+    } else if (p.m <= 16 && fits(g16, 512)) {
         fp8_gemm_rows_kernel<T, 1, 4><<<(unsigned)g16, 512, 0, s>>>(p);
     } else if (p.m <= 32 && fits(g16, 512)) {
         fp8_gemm_rows_kernel<T, 2, 2><<<(unsigned)g16, 512, 0, s>>>(p);
@@ -115,11 +122,6 @@ void launch_gemm(const GemmParams& p, float* work, int64_t work_bytes, hipStream
         if constexpr (!HALF) fp8_gemm_rows_kernel<T, 4, 2><<<(unsigned)g16, 512, 0, s>>>(p);
     } else if (!ring) {
         fp8_gemm64_kernel<T><<<(unsigned)t64, 256, 0, s>>>(p);
-    } else if (splits > 1) {
-        GemmParams q = p;
-        q.c = work;
-        fp8_gemm_ring_kernel<T, 2, 2, true><<<dim3((unsigned)t128, (unsigned)splits), 256, 0, s>>>(q, tiles(p.m, 128), tiles(p.n, 128));
-        join_splits_kernel<T><<<(unsigned)((p.m * p.n + 1023) / 1024), 256, 0, s>>>(p, work, splits);
     } else if (p.k >= 1024 && (t256 > 256 || (t256 >= 160 && p.k >= 2048))) {
         bool streamed = false;
         if constexpr (HALF) {

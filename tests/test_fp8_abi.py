@@ -48,7 +48,7 @@ def test_matmul_workspace(hip_lib):
     assert work(0, 5, 5, 0) == work(5, 0, 5, 0) == work(5, 5, 0, 0) == 0
     for m, n, k in ((1, 4096, 4096), (512, 1024, 1024), (65536, 1024, 1024), (8192, 8192, 8192), (4096, 4096, 16384)):
         assert work(m, n, k, 1) == 0 and work(m, n, k, 0) == 0
-    for m, n, k in ((1024, 1024, 65536), (145, 568, 17801), (256, 256, 100000)):
+    for m, n, k in ((1024, 1024, 65536), (145, 568, 17801), (256, 256, 100000), (9, 1024, 65536)):
         for dt in (0, 1, 2):
             parts, rest = divmod(work(m, n, k, dt), m * n * 4)
             assert rest == 0 and 2 <= parts <= 64 and parts <= k // 1024, (m, n, k, dt, parts)

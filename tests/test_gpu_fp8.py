@@ -224,7 +224,7 @@ def test_matmul_many_tiles(cuda_device, m, n, k, bias, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('m,n,k', [(145, 201, 17801), (130, 260, 8192)])
+@pytest.mark.parametrize('m,n,k', [(145, 201, 17801), (130, 260, 8192), (9, 300, 20000), (31, 130, 16400), (64, 64, 9000), (1, 5, 40000)])
 def test_matmul_cut(cuda_device, hip_lib, m, n, k, dtype):
     """Few tiles and a long k, shared by several workgroups: a strided output at an odd address with nothing around it written, the same
     bits on two streams at once and in a replayed graph, the uncut product without a workspace."""
