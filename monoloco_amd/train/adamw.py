@@ -73,16 +73,31 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr=1e
     torch.autograd.graph.increment_version(params)   # (LocoModel re-packs its engine when a parameter's version moved)
 
 
+def _check_group(g):
+    """A parameter group, given or loaded, that asks for this step and no other one."""
+    missing = [k for k in ('lr', 'betas', 'eps', 'weight_decay') if k not in g]
+    _need(not missing, "AdamW: a group without %s", ', '.join(missing))
+    _need(g.get('state_bits', 32) in (8, 32), "AdamW: moments have 8 or 32 bits, not %r", g.get('state_bits'))
+    _need(g['lr'] >= 0 and g['eps'] >= 0 and g['weight_decay'] >= 0 and all(0 <= b < 1 for b in g['betas']),
+          "AdamW: lr, eps and weight_decay are not negative, betas are in [0, 1)")
+    for flag in ('maximize', 'amsgrad'):
+        _need(not g.get(flag), "AdamW: %s is not supported", flag)
+    _need(g.get('decoupled_weight_decay', True) or not g['weight_decay'], "AdamW: the weight decay is decoupled from the gradient, a group asks for the other kind")
+
+
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW``'s arguments, groups, schedulers and state_dict on ``adamw_step``.
+    """``torch.optim.AdamW``'s arguments, groups, schedulers and state_dict on ``adamw_step``; groups that ask for ``maximize``, ``amsgrad``
+    or a decay through the gradient are refused.
 
     ``state_bits=8`` keeps the moments as e4m3 blocks (2 + 1/64 bytes per parameter instead of 8); ``seed`` is their rounding's.
     Parameters that got no gradient are left as they are, each counts its own steps."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
-        _need(state_bits in (8, 32), "AdamW: moments have 8 or 32 bits, not %r", state_bits)
-        _need(lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas), "AdamW: lr, eps and weight_decay are not negative, betas are in [0, 1)")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=int(seed)))
+
+    def add_param_group(self, param_group):
+        _check_group({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _state(self, p, bits):
         s = self.state[p]
@@ -118,12 +133,18 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments keep the types they were saved in (the base class casts them to the parameters').  A state_dict of
-        ``torch.optim.AdamW`` loads, too (moments in 32 bits)."""
+        ``torch.optim.AdamW`` loads, too (moments in 32 bits); what asks for another rule is refused before anything changes."""
         own = [{k: g[k] for k in ('state_bits', 'seed')} for g in self.param_groups]
         saved_groups = state_dict['param_groups']
         for mine, saved in zip(own, saved_groups):
             bits = saved.get('state_bits', 32)
             _need(bits == mine['state_bits'], "AdamW: the saved moments have %d bits, this optimizer's %d", bits, mine['state_bits'])
+        for g in saved_groups:
+            _check_group(g)
+            need = {'step', 'exp_avg', 'exp_avg_sq'} | ({'scales'} if g.get('state_bits', 32) == 8 else set())
+            for i in g['params']:
+                keys = set(state_dict['state'].get(i) or need)
+                _need(need <= keys <= need | {'max_exp_avg_sq'}, "AdamW: the state of another optimizer: %s", sorted(keys))
         super().load_state_dict(state_dict)
         ids = [i for g in saved_groups for i in g['params']]
         for g, mine in zip(self.param_groups, own):

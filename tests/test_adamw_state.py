@@ -1,0 +1,65 @@
+"""AdamW's groups and state on the CPU: what it cannot honour is refused, with nothing changed (no GPU: no step is launched)."""
+import copy
+
+import pytest
+import torch
+
+from monoloco_amd.train import AdamW
+
+
+def params(k=2):
+    return [torch.nn.Parameter(torch.full((3,), float(i))) for i in range(k)]
+
+
+def stepped(cls, **kw):
+    ps = params()
+    o = cls(ps, lr=0.5, **kw)
+    for p in ps:
+        p.grad = torch.ones(3)
+    o.step()
+    return o.state_dict()
+
+
+def refused(own, saved, text):
+    before = copy.deepcopy(own.state_dict())
+    with pytest.raises(ValueError, match=text):
+        own.load_state_dict(copy.deepcopy(saved))
+    assert own.state_dict() == before and not own.state
+
+
+@pytest.mark.parametrize('cls,kw,text', [(torch.optim.AdamW, dict(maximize=True), 'maximize'), (torch.optim.AdamW, dict(amsgrad=True), 'amsgrad'),
+                                         (torch.optim.Adam, dict(maximize=True), 'maximize'), (torch.optim.Adam, dict(weight_decay=0.1), 'decay'),
+                                         (torch.optim.SGD, dict(momentum=0.9), 'betas'), (torch.optim.NAdam, {}, 'another'), (torch.optim.Adamax, {}, 'another')])
+def test_states_of_other_rules_are_refused(cls, kw, text):
+    refused(AdamW(params(), lr=0.25), stepped(cls, **kw), text)
+
+
+def test_the_last_group_counts_too():
+    ps = params()
+    o = torch.optim.AdamW([{'params': ps[:1]}, {'params': ps[1:], 'maximize': True}])
+    qs = params()
+    refused(AdamW([{'params': qs[:1]}, {'params': qs[1:]}]), o.state_dict(), 'maximize')
+
+
+def test_states_of_the_same_rule_load():
+    for cls, kw in ((torch.optim.AdamW, {}), (torch.optim.Adam, {}), (torch.optim.AdamW, dict(foreach=True, weight_decay=0.1))):
+        saved = stepped(cls, **kw)
+        o = AdamW(params(), state_bits=32, seed=5)
+        o.load_state_dict(saved)
+        g = o.param_groups[0]
+        assert g['lr'] == 0.5 and g['weight_decay'] == saved['param_groups'][0]['weight_decay'] and (g['state_bits'], g['seed']) == (32, 5)
+        for i, p in enumerate(g['params']):
+            assert o.state[p]['step'] == 1 and all(torch.equal(o.state[p][k], saved['state'][i][k]) for k in ('exp_avg', 'exp_avg_sq'))
+
+
+@pytest.mark.parametrize('kw,text', [(dict(maximize=True), 'maximize'), (dict(amsgrad=True), 'amsgrad'), (dict(decoupled_weight_decay=False), 'decay'),
+                                     (dict(state_bits=16), 'bits'), (dict(betas=(0.9, 1.0)), 'betas'), (dict(lr=-1.0), 'lr')])
+def test_groups_are_checked(kw, text):
+    with pytest.raises(ValueError, match=text):
+        AdamW([{'params': params(1)}, {'params': params(1), **kw}])
+    o = AdamW(params(1))
+    with pytest.raises(ValueError, match=text):
+        o.add_param_group({'params': params(1), **kw})
+    assert len(o.param_groups) == 1
+    o.add_param_group({'params': params(1), 'state_bits': 8, 'maximize': False, 'name': 'last'})
+    assert o.param_groups[1]['name'] == 'last' and o.param_groups[1]['seed'] == 0
