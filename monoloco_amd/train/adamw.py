@@ -89,7 +89,8 @@ class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW``'s arguments, groups, schedulers and state_dict on ``adamw_step``; groups that ask for ``maximize``, ``amsgrad``
     or a decay through the gradient are refused.
 
-    ``state_bits=8`` keeps the moments as e4m3 blocks (2 + 1/64 bytes per parameter instead of 8); ``seed`` is their rounding's.
+    ``state_bits=8`` keeps the moments as e4m3 blocks (2 + 1/64 bytes per parameter instead of 8); ``seed`` is their rounding's: each
+    tensor of an optimizer has random bits of its own, two optimizers take two seeds.
     Parameters that got no gradient are left as they are, each counts its own steps."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
@@ -109,26 +110,49 @@ class AdamW(torch.optim.Optimizer):
                 s['scales'] = state_scales(p.numel(), p.device)
         return s
 
+    @staticmethod
+    def _in_place(lists, places):
+        """The lists with tensors without elements wherever a place has none (the library skips them, but counts them)."""
+        out = []
+        for ts in lists:
+            none = ts[0].new_empty(ts[0].shape[:1] + (0,) if ts is lists[4] else 0)
+            full = [none] * (places[-1] + 1)
+            for i, t in zip(places, ts):
+                full[i] = t
+            out.append(full)
+        return out
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            calls, bits = {}, group['state_bits']
+        for place, group in enumerate(self.param_groups):
+            bits, kinds = group['state_bits'], {}
             for p in group['params']:
-                if p.grad is None:
-                    continue
-                _need(not p.grad.is_sparse, "AdamW: sparse gradients are not supported")
-                s = self._state(p, bits)
-                calls.setdefault((p.device, p.dtype, s['step'] + 1), []).append((p, s))
-            for (_, _, step), found in calls.items():
-                adamw_step([p for p, _ in found], [p.grad for p, _ in found], [s['exp_avg'] for _, s in found], [s['exp_avg_sq'] for _, s in found],
-                           [s['scales'] for _, s in found] if bits == 8 else None, step=step, lr=float(group['lr']), betas=group['betas'],
-                           eps=group['eps'], weight_decay=group['weight_decay'], seed=group['seed'])
-                for _, s in found:
-                    s['step'] = step
+                kinds.setdefault((p.device, p.dtype), []).append(p)
+            for kind, ps in enumerate(kinds.values()):
+                # random bits go by seed, step and place in the call: a seed of its own for every call of a step, and (below) a place for
+                # every tensor that does not depend on which of the others have a gradient
+                seed = (group['seed'] + 0x9e3779b9 * place + 0x85ebca6b * kind) & 0xffffffff
+                calls = {}
+                for i, p in enumerate(ps):
+                    if p.grad is None:
+                        continue
+                    _need(not p.grad.is_sparse, "AdamW: sparse gradients are not supported")
+                    s = self._state(p, bits)
+                    calls.setdefault(s['step'] + 1, []).append((i, p, s))
+                for step, found in calls.items():
+                    lists = [[p for _, p, _ in found], [p.grad for _, p, _ in found], [s['exp_avg'] for _, _, s in found], [s['exp_avg_sq'] for _, _, s in found]]
+                    if bits == 8:
+                        lists.append([s['scales'] for _, _, s in found])
+                        if found[-1][0] >= len(found):
+                            lists = self._in_place(lists, [i for i, _, _ in found])
+                    adamw_step(*lists[:4], lists[4] if bits == 8 else None, step=step, lr=float(group['lr']), betas=group['betas'], eps=group['eps'],
+                               weight_decay=group['weight_decay'], seed=seed)
+                    for _, _, s in found:
+                        s['step'] = step
         return loss
 
     def load_state_dict(self, state_dict):

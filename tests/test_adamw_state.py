@@ -63,3 +63,32 @@ def test_groups_are_checked(kw, text):
     assert len(o.param_groups) == 1
     o.add_param_group({'params': params(1), 'state_bits': 8, 'maximize': False, 'name': 'last'})
     assert o.param_groups[1]['name'] == 'last' and o.param_groups[1]['seed'] == 0
+
+
+def test_no_two_tensors_share_random_bits(monkeypatch):
+    """The bits follow from (seed, step, place in the call): over groups, types and parameters that lag behind (no gradient for some steps) no
+    two tensors ever meet with the same three, and a tensor's place does not depend on which of the others have gradients."""
+    import monoloco_amd.train.adamw as A
+    calls = []
+
+    def record(ps, gs, ms, vs, scales, *, step, seed, **_):
+        assert len(ps) == len(gs) == len(ms) == len(vs) == len(scales)
+        calls.extend((seed, step, i, p) for i, p in enumerate(ps) if p.numel())
+
+    monkeypatch.setattr(A, 'adamw_step', record)
+    ps = params(6) + [torch.nn.Parameter(torch.zeros(3, dtype=torch.bfloat16)) for _ in range(3)]
+    groups = [[ps[0], ps[1], ps[6], ps[2]], [ps[3], ps[7]], [ps[4], ps[8], ps[5]]]
+    o = AdamW([{'params': g} for g in groups], state_bits=8, seed=77)
+    seen, places = {}, {}
+    for it in range(6):
+        for k, p in enumerate(ps):
+            p.grad = None if (k + it) % 3 == 0 else torch.ones_like(p)
+        calls.clear()
+        o.step()
+        assert {id(c[3]) for c in calls} == {id(p) for p in ps if p.grad is not None} and len(calls) == 6
+        for seed, step, i, p in calls:
+            assert seen.setdefault((seed, step, i), id(p)) == id(p)
+            assert places.setdefault(id(p), (seed, i)) == (seed, i)
+            assert o.state[p]['step'] == step
+    assert places[id(ps[0])] == (77, 0) and places[id(ps[1])] == (77, 1)       # the first tensors: as adamw_step with the same seed
+    assert all(0 <= s < 1 << 32 for s, _ in places.values())
