@@ -194,9 +194,10 @@ def _linear_sizes(m, n, k, need_dx, need_dw, need_db):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, grads):
         n, k = weight.shape
-        need_x, need_w, need_b = ctx.needs_input_grad
+        # (needs_input_grad is requires_grad alone, also where gradients are off)
+        need_x, need_w, need_b = (grads and need for need in ctx.needs_input_grad[:3])
         x2, w2 = _flat_rows(x, k), _rows(weight)
         m = x2.shape[0]
         dev = x.device
@@ -214,7 +215,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        want_x, want_w, want_b = ctx.needs_input_grad
+        want_x, want_w, want_b, _ = ctx.needs_input_grad
         saved, = ctx.saved_tensors
         m, n, k, need_x, need_w, xshape, xdt, wdt, bdt = ctx.was
         dev = dy.device
@@ -229,7 +230,7 @@ class _Linear(torch.autograd.Function):
                  DTYPES[bdt] if want_b else 0, m, n, k, need_x, need_w, work.data_ptr())
         elif want_x:
             dx.zero_()
-        return dx, dw, db
+        return dx, dw, db, None
 
 
 def linear(x, weight, bias=None):
@@ -237,7 +238,8 @@ def linear(x, weight, bias=None):
 
     Forward: x in 1 x 128 blocks of its rows, the weight in 128 x 128 tiles.  Backward, from dy rounded the same way: dx from the
     transposed tiles of the weight, dw from dy^T and x^T in 1 x 128 blocks along the batch, the bias gradient from dy itself.  What is kept
-    for the backward pass are the 8-bit transposed operands, not x.  x, weight and bias may each be fp32, bf16 or fp16."""
+    for the backward pass are the 8-bit transposed operands, not x (without gradients nothing is prepared or kept; the weight is still
+    quantised in every call: ``quantize`` it once and use ``matmul`` to serve).  x, weight and bias may each be fp32, bf16 or fp16."""
     _device_of('linear', x, weight, bias)
     if not (x.dim() and weight.dim() == 2 and x.shape[-1] == weight.shape[1]):
         raise ValueError("linear: x %s does not fit weight %s" % (tuple(x.shape), tuple(weight.shape)))
@@ -250,7 +252,7 @@ def linear(x, weight, bias=None):
             raise ValueError("linear: the bias is (%d) in fp32, bf16 or fp16, got %s %s" % (weight.shape[0], tuple(bias.shape), bias.dtype))
         if not bias.is_contiguous():
             bias = bias.contiguous()
-    return _Linear.apply(x, weight, bias)
+    return _Linear.apply(x, weight, bias, torch.is_grad_enabled())
 
 
 def _norm_args(name, x, weight, residual, eps):
