@@ -205,9 +205,11 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
     if (lda < k || ldb < k || ldc < n || ldsa < kb || ldsb < kb) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: a row stride is shorter than its row");
     const long grid = ((m + 63) / 64) * ((n + 63) / 64);
     if (m > (1LL << 40) || n > (1LL << 33) || !fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
-    GemmParams p{a_dev, b_dev, a_scale_dev, b_scale_dev, (long)lda, (long)ldb, (long)ldsa, (long)ldsb, a_tile != 0, b_tile != 0, bias_dev, bias_dtype, c_dev,
+    // (the stride of a single row is never taken: whatever it is, it must not decide which kernel runs)
+    const long la = m > 1 ? lda : 0, lb = n > 1 ? ldb : 0;
+    GemmParams p{a_dev, b_dev, a_scale_dev, b_scale_dev, la, lb, (long)ldsa, (long)ldsb, a_tile != 0, b_tile != 0, bias_dev, bias_dtype, c_dev,
                  (long)m, (long)n, (long)k, (long)ldc, 0, 0};
-    p.fast_a = rows_aligned(a_dev, lda, 1, 16), p.fast_b = rows_aligned(b_dev, ldb, 1, 16);
+    p.fast_a = rows_aligned(a_dev, la, 1, 16), p.fast_b = rows_aligned(b_dev, lb, 1, 16);
     const hipStream_t s = (hipStream_t)stream;
     with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, (float*)work_dev, work_bytes, s); });
     return ops_launched("ml_fp8_matmul");
