@@ -467,7 +467,7 @@ int64_t ml_rms_norm_backward_groups(int64_t m, int64_t n);
 int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int64_t ldh, const void* dh_dev, int64_t ldd, int dtype,
                          const void* w_dev, int w_dtype, int64_t m, int64_t n, float eps, void* dx_dev, int64_t ldx, void* dw_dev,
                          float* work_dev, void* stream);
-/* out (n) of `dtype` = sum over the rows of part (rows, n), fp32, in a fixed order. */
+/* out (n) of `dtype` = sum over the rows of part (rows, n), fp32, summed in 64 bits in a fixed order and rounded once. */
 int ml_sum_rows(const float* part_dev, int64_t rows, int64_t n, void* out_dev, int dtype, void* stream);
 /* One AdamW step, in place, over n_tensors contiguous tensors of one dtype that do not overlap (the reference's optimizer is torch's Adam,
  * monoloco/train/trainer.py:128):  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;

@@ -325,7 +325,7 @@ int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int
     if (n == 0) return ML_OK;
     if (!dw_dev || (m > 0 && (!dy_dev || !h_dev || !w_dev || !dx_dev || !work_dev))) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: null pointer");
     if (m > 0 && (ldy < n || ldh < n || (dh_dev && ldd < n) || ldx < n)) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: a row stride is shorter than its row");
-    if (!fits((n + 31) / 32, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm_backward: %lld columns are too many", (long long)n);
+    if (!fits((n + REDUCE_COLS - 1) / REDUCE_COLS, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm_backward: %lld columns are too many", (long long)n);
     const hipStream_t s = (hipStream_t)stream;
     const long groups = m ? norm_groups(m, n) : 0;
     if (m > 0) {
@@ -336,7 +336,7 @@ int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int
         const int rc = ops_launched("ml_rms_norm_backward");
         if (rc) return rc;
     }
-    with_type(w_dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + 31) / 32), 1024, 0, s>>>(work_dev, groups, n, (decltype(t)*)dw_dev); });
+    with_type(w_dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + REDUCE_COLS - 1) / REDUCE_COLS), 1024, 0, s>>>(work_dev, groups, n, (decltype(t)*)dw_dev); });
     return ops_launched("ml_rms_norm_backward");
 }
 
@@ -344,8 +344,8 @@ int ml_sum_rows(const float* part_dev, int64_t rows, int64_t n, void* out_dev, i
     if (!elem_size(dtype) || rows < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_sum_rows: bad type %d or size", dtype);
     if (n == 0) return ML_OK;
     if (!out_dev || (rows > 0 && !part_dev)) return ops_fail(ML_ERR_ARG, "ml_sum_rows: null pointer");
-    if (!fits((n + 31) / 32, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_sum_rows: %lld columns are too many", (long long)n);
-    with_type(dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + 31) / 32), 1024, 0, (hipStream_t)stream>>>(part_dev, rows, n, (decltype(t)*)out_dev); });
+    if (!fits((n + REDUCE_COLS - 1) / REDUCE_COLS, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_sum_rows: %lld columns are too many", (long long)n);
+    with_type(dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + REDUCE_COLS - 1) / REDUCE_COLS), 1024, 0, (hipStream_t)stream>>>(part_dev, rows, n, (decltype(t)*)out_dev); });
     return ops_launched("ml_sum_rows");
 }
 

@@ -260,28 +260,33 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
     }
 }
 
-// out[c] = sum over g of part[g * n + c], in a fixed order: 32 columns per workgroup, 32 teams take g = t, t + 32, ..., eight loads of
-// each in flight (one after the other they cost 11 us for 1024 x 1024)
+// out[c] = sum over g of part[g * n + c] in 64 bits (in 32 the join alone rounded as often as all sums before it), in a fixed order: COLS
+// columns per workgroup, 1024 / COLS teams take g = t, t + teams, ..., eight loads of each in flight.  1024 x 1024: 3.9 us (loads one after
+// the other: 11; 64-bit sums with 32 columns: 5.8, with 8: 3.1, but 12.9 instead of 4.6 for 512 x 8192; 32-bit sums: 3.6).
+constexpr int REDUCE_COLS = 16;
 template <typename T>
 __global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restrict__ part, long groups, long n, T* __restrict__ out) {
-    __shared__ float s[32][33];
-    const int cx = threadIdx.x & 31, t = threadIdx.x >> 5;
-    const long c = (long)blockIdx.x * 32 + cx;
-    float a = 0.0f;
+    constexpr int COLS = REDUCE_COLS, TEAMS = 1024 / COLS;
+    __shared__ double s[16][COLS];
+    const int cx = threadIdx.x % COLS, t = threadIdx.x / COLS;
+    const long c = (long)blockIdx.x * COLS + cx;
+    double a = 0.0;
     if (c < n)
-        for (long g = t; g < groups; g += 256) {
+        for (long g = t; g < groups; g += 8 * TEAMS) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = g + 32 * u < groups ? part[(g + 32 * u) * n + c] : 0.0f;
-            a += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            for (int u = 0; u < 8; ++u) v[u] = g + TEAMS * u < groups ? part[(g + TEAMS * u) * n + c] : 0.0f;
+            a += (((double)v[0] + v[1]) + ((double)v[2] + v[3])) + (((double)v[4] + v[5]) + ((double)v[6] + v[7]));
         }
-    s[t][cx] = a;
+#pragma unroll
+    for (int d = COLS; d < 64; d *= 2) a += __shfl_xor(a, d);   // the wave's teams
+    if ((threadIdx.x & 63) < COLS) s[threadIdx.x >> 6][cx] = a;
     __syncthreads();
     if (t == 0 && c < n) {
-        float v = 0.0f;
+        double v[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v += s[i][cx];
-        out[c] = (T)v;
+        for (int i = 0; i < 16; ++i) v[i & 3] += s[i][cx];
+        out[c] = (T)((v[0] + v[1]) + (v[2] + v[3]));
     }
 }
 
