@@ -469,8 +469,8 @@ int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int
                          float* work_dev, void* stream);
 /* out (n) of `dtype` = sum over the rows of part (rows, n), fp32, summed in 64 bits in a fixed order and rounded once. */
 int ml_sum_rows(const float* part_dev, int64_t rows, int64_t n, void* out_dev, int dtype, void* stream);
-/* One AdamW step, in place, over n_tensors contiguous tensors of one dtype that do not overlap (the reference's optimizer is torch's Adam,
- * monoloco/train/trainer.py:128):  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+/* One AdamW step, in place, over n_tensors contiguous tensors of one dtype; arrays that share memory are refused (a gradient may be one of its
+ * own tensor's arrays; the reference's optimizer is torch's Adam, monoloco/train/trainer.py:128):  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
  * p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps).  Host arrays of device pointers; they may be reused as
  * soon as the call returns.  scales == NULL: exp_avgs / exp_avg_sqs are fp32.  Otherwise they are e4m3 codes of m and of sqrt(v) in blocks of
  * 128 along the flattened tensor, scales[i] holds ceil(numel / 128) bytes for m, then as many for sqrt(v), and both are rounded

@@ -31,6 +31,8 @@ ML_DEBUG_MID_SPLIT4 = 16384
 ML_DEBUG_MID_NODMA = 32768
 ML_FLAG_MERGE_W2W3 = 1
 ML_FLAG_HOST_ONLY = 256
+ML_ERR_ARG = 1
+ML_ERR_SHAPE = 4
 ML_F32 = 0
 ML_BF16 = 1
 ML_F16 = 2
@@ -42,6 +44,10 @@ OUT_COLS = dict(x=0, y=1, z=2, d=3, bi=4, yaw=5, yaw_ego=6, aux=7, h=8, w=9, l=1
 
 class MonolocoHipError(RuntimeError):
     """Raised when the HIP library is missing or one of its entry points reports an error."""
+
+
+class MonolocoArgumentError(MonolocoHipError, ValueError):
+    """Raised where an operator's entry point refuses its arguments or their sizes."""
 
 
 # name -> (restype, argtypes); must list every symbol of include/monoloco_hip.h
@@ -192,7 +198,8 @@ def check_ops(code):
     """check() for the 8-bit residual-block operators (their error text is ml_ops_last_error's)."""
     if code != 0:
         msg = load().ml_ops_last_error()
-        raise MonolocoHipError("monoloco_hip error %d: %s" % (code, msg.decode() if msg else '?'))
+        kind = MonolocoArgumentError if code in (ML_ERR_ARG, ML_ERR_SHAPE) else MonolocoHipError
+        raise kind("monoloco_hip error %d: %s" % (code, msg.decode() if msg else '?'))
 
 
 def fptr(array):

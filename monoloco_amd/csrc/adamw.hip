@@ -13,6 +13,10 @@
 // element alone (rng.h's generator).  The update itself uses the unrounded m' and r'.  r' > 0 keeps at least the smallest code: a
 // second moment that vanished would let the next step divide by eps.  (eps = 0 and a second moment below fp32's normal range: the divisor
 // is taken as the smallest normal number.)
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "block8.h"
 #include "rng.h"
 
@@ -30,7 +34,7 @@ struct AdamTable {
     uint8_t* s[MAX_TENSORS];        // 8-bit moments: scales of m, then of r (blocks each)
     long numel[MAX_TENSORS];
     unsigned first[MAX_TENSORS];    // first workgroup of the tensor; behind the last tensor: the grid
-    unsigned key[MAX_TENSORS];      // random key of the tensor; 
+    unsigned key[MAX_TENSORS];      // random key of the tensor
 };
 static_assert(sizeof(AdamTable) <= 3700, "kernel arguments");
 
@@ -196,6 +200,32 @@ uint32_t host_mix32(uint32_t x) {
     return x ^ (x >> 16);
 }
 
+// All tensors of a call are written side by side: memory that two of them share, in whole or in part, would be a race.  A gradient may be
+// one of its own tensor's arrays (every element is read before it is written), nothing else that is written.  (152 arrays: 4 us.)
+int check_apart(int n, const int64_t* numel, void* const* p, const void* const* g, int es, void* const* m, void* const* v, int ms, uint8_t* const* scales) {
+    struct Span { uintptr_t from, to; int tensor; };
+    std::vector<Span> w;
+    w.reserve((size_t)n * 4);
+    for (int i = 0; i < n; ++i) {
+        if (numel[i] == 0) continue;
+        auto add = [&](const void* at, int64_t bytes) { w.push_back({(uintptr_t)at, (uintptr_t)at + (uintptr_t)bytes, i}); };
+        add(p[i], numel[i] * es), add(m[i], numel[i] * ms), add(v[i], numel[i] * ms);
+        if (scales) add(scales[i], (numel[i] + QB - 1) / QB * 2);
+    }
+    std::sort(w.begin(), w.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+    for (size_t i = 1; i < w.size(); ++i)
+        if (w[i].from < w[i - 1].to) return ops_fail(ML_ERR_ARG, "ml_adamw_step: a tensor is given twice, or tensors share memory (%d and %d)", std::min(w[i - 1].tensor, w[i].tensor),
+                                                         std::max(w[i - 1].tensor, w[i].tensor));
+    for (int i = 0; i < n; ++i) {
+        if (numel[i] == 0) continue;
+        const uintptr_t from = (uintptr_t)g[i], to = from + (uintptr_t)numel[i] * es;
+        const auto at = std::upper_bound(w.begin(), w.end(), from, [](uintptr_t x, const Span& b) { return x < b.to; });
+        if (at != w.end() && at->from < to && !(at->tensor == i && at->from == from && at->to == to))
+            return ops_fail(ML_ERR_ARG, "ml_adamw_step: gradient %d shares memory with what the step writes of tensor %d", i, at->tensor);
+    }
+    return ML_OK;
+}
+
 }  // namespace
 
 extern "C" int ml_adamw_step(int n_tensors, const int64_t* numel, void* const* params, const void* const* grads, int dtype, void* const* exp_avgs,
@@ -209,6 +239,12 @@ extern "C" int ml_adamw_step(int n_tensors, const int64_t* numel, void* const* p
     for (int i = 0; i < n_tensors; ++i) {
         if (numel[i] < 0 || numel[i] > (1LL << 35)) return ops_fail(ML_ERR_SHAPE, "ml_adamw_step: tensor %d has %lld elements", i, (long long)numel[i]);
         if (numel[i] && (!params[i] || !grads[i] || !exp_avgs[i] || !exp_avg_sqs[i] || (scales && !scales[i]))) return ops_fail(ML_ERR_ARG, "ml_adamw_step: tensor %d has a null pointer", i);
+    }
+    try {
+        const int rc = check_apart(n_tensors, numel, params, grads, dtype == ML_F32 ? 4 : 2, exp_avgs, exp_avg_sqs, scales ? 1 : 4, scales);
+        if (rc) return rc;
+    } catch (const std::bad_alloc&) {
+        return ops_fail(ML_ERR_STATE, "ml_adamw_step: no host memory for %d tensors", n_tensors);
     }
     const hipStream_t s = (hipStream_t)stream;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;

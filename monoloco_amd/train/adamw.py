@@ -25,7 +25,8 @@ def state_scales(numel, device):
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, seed=0):
-    """One AdamW step in place: ``step`` counts from 1, all tensors of one type (fp32, bf16, fp16) and device, contiguous, none twice.
+    """One AdamW step in place: ``step`` counts from 1, all tensors of one type (fp32, bf16, fp16) and device, contiguous,
+    none twice and none sharing memory with another (refused).
 
     Without ``scales`` the moments are fp32 tensors like the parameters.  With ``scales`` (one (2, ceil(numel / 128)) tensor of e8m0 for
     each parameter, see ``state_scales``) they are e4m3 codes: exp_avgs of the first moment, exp_avg_sqs of the ROOT of the second, both
@@ -62,10 +63,6 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales=None, *, step, lr=1e
                                  % (n, -(-n // BLOCK), SCALES, index, tuple(s.shape), s.dtype, s.device))
     ps, gs, ms, vs = (array('Q', map(_T.data_ptr, ts)) for ts in (params, grads, exp_avgs, exp_avg_sqs))
     ss = array('Q', map(_T.data_ptr, scales)) if scales is not None else None
-    written = {*ps, *ms, *vs}
-    if len(written) != 3 * k:
-        written = [a for ts in (ps, ms, vs) for a, n in zip(ts, sizes) if n]
-        _need(len(set(written)) == len(written), "adamw_step: a tensor is given twice")
     numel = array('q', sizes)
     _run(index, _lib.load().ml_adamw_step, k, _address(numel), _address(ps), _address(gs),
          DTYPES[dt], _address(ms), _address(vs), None if ss is None else _address(ss), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps),

@@ -92,3 +92,47 @@ def test_no_two_tensors_share_random_bits(monkeypatch):
             assert o.state[p]['step'] == step
     assert places[id(ps[0])] == (77, 0) and places[id(ps[1])] == (77, 1)       # the first tensors: as adamw_step with the same seed
     assert all(0 <= s < 1 << 32 for s, _ in places.values())
+
+
+def test_shared_memory_is_refused(hip_lib):
+    """Decided on the host, before any HIP call (no pointer here is ever used: every call is refused)."""
+    import ctypes
+
+    def call(text, eight=False, dtype=0, **move):
+        n = 3
+        numel = [128, 0, 300]
+        at = {k: [0x10000 * (1 + 4 * j), 0, 0x10000 * (2 + 4 * j)] for j, k in enumerate(('p', 'g', 'm', 'v', 's'))}
+        for k, (i, a) in move.items():
+            at[k][i] = a
+        arr = lambda k: (ctypes.c_void_p * n)(*[a or None for a in at[k]])  # noqa: E731
+        assert hip_lib.ml_adamw_step(n, (ctypes.c_int64 * n)(*numel), arr('p'), arr('g'), dtype, arr('m'), arr('v'), arr('s') if eight else None, 1, 1e-3, 0.9,
+                                     0.999, 1e-8, 0.01, 0, None) == 1
+        assert text in hip_lib.ml_ops_last_error().decode(), hip_lib.ml_ops_last_error()
+
+    p0, p2, m0, s0 = 0x10000, 0x20000, 0x90000, 0x110000
+    both = 'given twice, or tensors share memory (0 and 2)'
+    for eight in (False, True):
+        call(both, eight, p=(2, p0))                              # the same parameter
+        call(both, eight, p=(2, p0 + 128 * 4 - 4))                # its last element
+        call(both, eight, p=(2, p0 - 300 * 4 + 4))                # its first one
+        call(both, eight, dtype=1, p=(2, p0 + 128 * 2 - 2))
+        call(both, eight, v=(2, p0 + 8))
+        call('tensors share memory (0 and 0)', eight, m=(0, p0))
+        call('gradient 0 shares memory with what the step writes of tensor 2', eight, g=(0, p2))
+        call('gradient 2 shares memory with what the step writes of tensor 2', eight, g=(2, p2 + 4))
+        call('gradient 2 shares memory with what the step writes of tensor 0', eight, g=(2, m0 - 300 * 4 + 1))
+    call(both, True, s=(2, s0))                                   # the same scales
+    call(both, True, s=(2, s0 + 1))
+    call(both, True, s=(2, m0 + 127))
+
+
+def test_library_refusals_are_value_errors(hip_lib):
+    """Wrong arguments raise ValueError, whoever finds them."""
+    from monoloco_amd import _lib
+    assert hip_lib.ml_sum_rows(None, -1, 1, None, 0, None) == 1
+    with pytest.raises(ValueError, match='bad type') as e:
+        _lib.check_ops(1)
+    assert isinstance(e.value, _lib.MonolocoHipError)
+    with pytest.raises(_lib.MonolocoHipError) as e:
+        _lib.check_ops(2)
+    assert not isinstance(e.value, ValueError)

@@ -46,3 +46,29 @@ def test_a_missing_gradient_moves_no_other_tensor(cuda_device):
             assert float((off > 0).double().mean()) <= 0.01 and bool((off <= 1.001 * R.step_of(want)).all())    # (2^-16 of a step: see test_gpu_adamw.py)
     for x, y in zip(*got):
         assert all(torch.equal(s, t) for s, t in zip(x, y))
+
+
+def test_neighbours_and_shared_gradients(cuda_device):
+    """Tensors that touch without a byte between them, one gradient for two of them, a gradient that is its own parameter: allowed.  What shares
+    memory is refused and nothing is written."""
+    from monoloco_amd.train import adamw_step
+    flat, m, v = torch.ones(300, device=cuda_device), torch.zeros(300, device=cuda_device), torch.zeros(300, device=cuda_device)
+    g = torch.full((100,), 0.5, device=cuda_device)
+
+    def cut(t, at=(0, 100, 200)):
+        return [t[i:i + 100] for i in at]
+
+    def step(ps, gs):
+        adamw_step(ps, gs, cut(m), cut(v), step=1, lr=0.1, weight_decay=0.0)
+
+    # the first step moves by lr * sign(g), but for eps (1e-8 / 0.5) and roundings (20 u of 0.1)
+    step(cut(flat), [g, flat[100:200], g])
+    assert bool(((flat - 0.9).abs() <= 0.1 * (2e-8 + 20 * 2.0 ** -24) + 2 * 2.0 ** -24).all()) and bool((g == 0.5).all())
+    before = [t.clone() for t in (flat, m, v)]
+    for ps, gs in ((cut(flat, (0, 99, 200)), [g, g, g]), (cut(flat, (0, 0, 200)), [g, g, g]), (cut(flat), [g, flat[150:250], g]), (cut(flat), [g, m[:100], g])):
+        with pytest.raises(ValueError, match='memory'):
+            step(ps, gs)
+    s = torch.zeros(2, 1, device=cuda_device).to(torch.float8_e8m0fnu)
+    with pytest.raises(ValueError, match='memory'):
+        adamw_step(cut(flat)[:2], [g, g], *([t.to(torch.float8_e4m3fn) for t in cut(x)[:2]] for x in (m, v)), [s, s], step=1)
+    assert all(torch.equal(x, y) for x, y in zip(before, (flat, m, v)))
