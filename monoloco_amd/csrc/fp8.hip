@@ -14,6 +14,10 @@ namespace {
 // a launch has fewer than 2^32 threads
 bool fits(long workgroups, int threads) { return workgroups <= 0xffffffffL / threads; }
 
+// a matrix that memory could hold (2^46 elements, 2^40 along an axis); beyond it, sums and products of sizes would leave 64 bits
+bool holds(int64_t rows, int64_t cols) { return rows <= 1LL << 40 && cols <= 1LL << 40 && (rows == 0 || cols <= (1LL << 46) / rows); }
+bool holds(int64_t m, int64_t n, int64_t k) { return holds(m, n) && holds(m, k) && holds(n, k); }
+
 int elem_size(int dtype) { return dtype == ML_F32 ? 4 : dtype == ML_BF16 || dtype == ML_F16 ? 2 : 0; }
 
 bool rows_aligned(const void* p, long ld, int es, int to) { return !p || (((uintptr_t)p % to) == 0 && (ld * es) % to == 0); }
@@ -170,10 +174,10 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
     if (!es || m < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_fp8_quantize: bad type %d or size %lld x %lld", dtype, (long long)m, (long long)n);
     if (m == 0 || n == 0) return ML_OK;
     if (!x_dev || (!q_dev && !qt_dev) || (q_dev && !scale_dev) || (qt_dev && !scale_t_dev)) return ops_fail(ML_ERR_ARG, "ml_fp8_quantize: null pointer");
+    if (!holds(m, n)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_quantize: %lld x %lld is too large", (long long)m, (long long)n);
     const long nb = (n + QB - 1) / QB, mb = (m + QB - 1) / QB;
     if (ldx < n || (q_dev && (ldq < n || lds < nb)) || (qt_dev && (ldqt < m || ldst < mb)))
         return ops_fail(ML_ERR_ARG, "ml_fp8_quantize: a row stride is shorter than its row");
-    if (m > (1LL << 40) || n > (1LL << 40)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_quantize: %lld x %lld is too large", (long long)m, (long long)n);
     QuantParams p{};
     p.x = x_dev, p.m = m, p.n = n, p.ldx = ldx, p.tile = tile != 0;
     p.q = q_dev, p.scale = scale_dev, p.ldq = ldq, p.lds = lds;
@@ -191,7 +195,7 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
 }
 
 int64_t ml_fp8_matmul_work(int64_t m, int64_t n, int64_t k, int c_dtype) {
-    return m <= 0 || n <= 0 || k <= 0 || m > (1LL << 33) || n > (1LL << 33) ? 0 : gemm_work_bytes(m, n, k, c_dtype != ML_F32);
+    return m <= 0 || n <= 0 || k <= 0 || !holds(m, n, k) ? 0 : gemm_work_bytes(m, n, k, c_dtype != ML_F32);
 }
 
 int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
@@ -201,10 +205,11 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
     if (!es || (bias_dev && !elem_size(bias_dtype)) || m < 0 || n < 0 || k < 0) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: bad type %d, %d or size", c_dtype, bias_dtype);
     if (m == 0 || n == 0) return ML_OK;
     if (!c_dev || (k > 0 && (!a_dev || !b_dev || !a_scale_dev || !b_scale_dev))) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: null pointer");
+    if (!holds(m, n, k)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld x %lld is too large", (long long)m, (long long)n, (long long)k);
     const long kb = (k + QB - 1) / QB;
     if (lda < k || ldb < k || ldc < n || ldsa < kb || ldsb < kb) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: a row stride is shorter than its row");
     const long grid = ((m + 63) / 64) * ((n + 63) / 64);
-    if (m > (1LL << 40) || n > (1LL << 33) || !fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
+    if (!fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
     // (the stride of a single row is never taken: whatever it is, it must not decide which kernel runs)
     const long la = m > 1 ? lda : 0, lb = n > 1 ? ldb : 0;
     GemmParams p{a_dev, b_dev, a_scale_dev, b_scale_dev, la, lb, (long)ldsa, (long)ldsb, a_tile != 0, b_tile != 0, bias_dev, bias_dtype, c_dev,
@@ -246,7 +251,8 @@ struct LinearPlan {
 }  // namespace
 
 int ml_fp8_linear_sizes(int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, int need_db, int64_t* bytes3) {
-    if (m < 0 || n < 0 || k < 0 || m > (1LL << 40) || n > (1LL << 40) || k > (1LL << 40) || !bytes3) return ops_fail(ML_ERR_ARG, "ml_fp8_linear_sizes: bad size or null pointer");
+    if (m < 0 || n < 0 || k < 0 || !bytes3) return ops_fail(ML_ERR_ARG, "ml_fp8_linear_sizes: bad size or null pointer");
+    if (!holds(m, n, k)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_linear_sizes: %lld x %lld x %lld is too large", (long long)m, (long long)n, (long long)k);
     const LinearPlan l(m, n, k, need_dx, need_dw, need_db);
     bytes3[0] = l.forward, bytes3[1] = l.saved, bytes3[2] = l.backward;
     return ML_OK;
@@ -255,6 +261,7 @@ int ml_fp8_linear_sizes(int64_t m, int64_t n, int64_t k, int need_dx, int need_d
 int ml_fp8_linear(const void* x_dev, int x_dtype, int64_t ldx, const void* w_dev, int w_dtype, int64_t ldw, const void* bias_dev, int bias_dtype, void* y_dev,
                   int64_t ldy, int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, void* work_dev, void* saved_dev, void* stream) {
     if (m < 0 || n < 0 || k < 1) return ops_fail(ML_ERR_ARG, "ml_fp8_linear: bad size");
+    if (!holds(m, n, k)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_linear: %lld x %lld x %lld is too large", (long long)m, (long long)n, (long long)k);
     if ((m && n && !work_dev) || ((need_dx || need_dw) && n && !saved_dev)) return ops_fail(ML_ERR_ARG, "ml_fp8_linear: null workspace");
     const LinearPlan l(m, n, k, need_dx, need_dw, false);
     uint8_t *const wk = (uint8_t*)work_dev, *const sv = (uint8_t*)saved_dev;
@@ -271,6 +278,7 @@ int ml_fp8_linear(const void* x_dev, int x_dtype, int64_t ldx, const void* w_dev
 int ml_fp8_linear_backward(const void* dy_dev, int dy_dtype, int64_t ldy, const void* saved_dev, void* dx_dev, int dx_dtype, void* dw_dev, int dw_dtype, void* db_dev,
                            int db_dtype, int64_t m, int64_t n, int64_t k, int need_dx, int need_dw, void* work_dev, void* stream) {
     if (m < 0 || n < 0 || k < 1) return ops_fail(ML_ERR_ARG, "ml_fp8_linear_backward: bad size");
+    if (!holds(m, n, k)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_linear_backward: %lld x %lld x %lld is too large", (long long)m, (long long)n, (long long)k);
     // (the layout of `saved` goes by what the forward pass was asked for, the work by what is asked for now)
     const LinearPlan l(m, n, k, need_dx, need_dw, db_dev != nullptr);
     const bool dx = dx_dev != nullptr, dw = dw_dev != nullptr;
