@@ -437,7 +437,7 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
 /* c (m, n) = a (m, k) . b (n, k)^T [+ bias (n)] in fp32 accumulation, rounded once to c_dtype; a, b codes with scales per row block or
  * per tile (a_tile, b_tile).  k = 0 gives the bias (or zeros).  16-bit results come from the 8-bit matrix instructions (1.5e-5 of the result's
  * norm, far below their rounding), fp32 results from exact bf16 operands at half the rate (4e-8); there the values that the operands stand
- * for have to lie in fp32's normal range (smaller ones count as 0). */
+ * for have to lie in fp32's normal range (smaller ones count as 0).  c may not share memory with what the call reads (refused). */
 int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
                   const uint8_t* b_scale_dev, int64_t ldsb, int b_tile, const void* bias_dev, int bias_dtype, void* c_dev, int c_dtype,
                   int64_t ldc, int64_t m, int64_t n, int64_t k, void* work_dev, int64_t work_bytes, void* stream);
@@ -514,6 +514,8 @@ int ml_debug_get_layer(const ml_loco* h, int layer, float* w_host, float* b_host
 int ml_debug_num_layers(const ml_loco* h);
 /* How many ml_loco_frame_mono calls of this process ran without any copy operation (pinned buffers, <= 128 persons). */
 long long ml_debug_frames_without_copies(void);
+/* Host only: do two areas of `rows` runs of `width` bytes, `pitch` apart, share no byte (what ml_fp8_matmul asks of c and its operands)? */
+int ml_debug_areas_apart(int64_t at, int64_t pitch, int64_t width, int64_t rows, int64_t at2, int64_t pitch2, int64_t width2, int64_t rows2);
 /* ml_loco_frame_mono, single image in pinned buffers: the host learns of the frame's end from a word of pinned memory the last
  * launch releases (busy-polled for at most 5 ms, then hipStreamSynchronize) instead of sleeping in the stream synchronisation.
  * enable 0 / 1 turns that off / on for the process (< 0: unchanged); returns how many frames have timed out so far (expected 0). */

@@ -147,6 +147,7 @@ SIGNATURES = {
     'ml_adamw_step': (c_int, [c_int, _P, _P, _P, c_int, _P, _P, _P, c_int64, c_double, c_double, c_double, c_double, c_double, c_uint32,
                               _P]),
     'ml_ops_last_error': (c_char_p, []),
+    'ml_debug_areas_apart': (c_int, [c_int64] * 8),
     'ml_loco_profile_begin': (c_int, [_P, c_int]),
     'ml_loco_profile_end': (c_int, [_P, POINTER(c_int64), POINTER(c_double), POINTER(c_double), POINTER(c_int64), c_int]),
     'ml_debug_linear': (c_int, [_P, c_int64, c_int, POINTER(c_float), POINTER(c_float), c_int, c_int, _P, _P,

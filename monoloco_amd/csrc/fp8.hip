@@ -22,6 +22,25 @@ int elem_size(int dtype) { return dtype == ML_F32 ? 4 : dtype == ML_BF16 || dtyp
 
 bool rows_aligned(const void* p, long ld, int es, int to) { return !p || (((uintptr_t)p % to) == 0 && (ld * es) % to == 0); }
 
+// `rows` runs of `width` bytes, `pitch` apart
+struct Area { int64_t at, pitch, width, rows; };
+// Do a result and an operand share no byte?  Exact where the operand is one run or both have the same pitch (columns of one buffer); runs
+// of different pitches that interleave count as shared.
+bool apart(const Area& c, const Area& t) {
+    if (c.rows <= 0 || c.width <= 0 || t.rows <= 0 || t.width <= 0) return true;
+    auto end = [](const Area& x) { return (__int128)x.at + (__int128)(x.rows - 1) * x.pitch + x.width; };
+    if (end(c) <= t.at || end(t) <= c.at) return true;
+    const int64_t d = t.at - c.at;
+    if (t.rows == 1) {   // the first run of c that ends behind t's start: does it start behind t's end?
+        const int64_t r = c.rows == 1 || d < c.width ? 0 : (d - c.width) / c.pitch + 1;
+        return r >= c.rows || (__int128)r * c.pitch >= (__int128)d + t.width;
+    }
+    if (c.rows == 1) return apart(t, c);
+    if (c.pitch != t.pitch) return false;
+    const int64_t x = (d % c.pitch + c.pitch) % c.pitch;
+    return x >= c.width && x + t.width <= c.pitch;
+}
+
 // f(T{}) for the element type
 template <typename F>
 void with_type(int dtype, F f) {
@@ -210,6 +229,12 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
     if (lda < k || ldb < k || ldc < n || ldsa < kb || ldsb < kb) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: a row stride is shorter than its row");
     const long grid = ((m + 63) / 64) * ((n + 63) / 64);
     if (!fits(grid, 256)) return ops_fail(ML_ERR_SHAPE, "ml_fp8_matmul: %lld x %lld is too large", (long long)m, (long long)n);
+    const Area c{(int64_t)(uintptr_t)c_dev, ldc * es, n * es, m};
+    auto area = [](const void* at, int64_t ld, int64_t width, int64_t rows) { return Area{(int64_t)(uintptr_t)at, ld, width, rows}; };
+    const char* const shared = !apart(c, area(a_dev, lda, k, m)) ? "a" : !apart(c, area(b_dev, ldb, k, n)) ? "b"
+                               : !apart(c, area(a_scale_dev, ldsa, kb, a_tile ? (m + QB - 1) / QB : m)) || !apart(c, area(b_scale_dev, ldsb, kb, b_tile ? (n + QB - 1) / QB : n)) ? "scales"
+                               : bias_dev && !apart(c, area(bias_dev, 0, n * elem_size(bias_dtype), 1)) ? "bias" : nullptr;
+    if (shared) return ops_fail(ML_ERR_ARG, "ml_fp8_matmul: the result shares memory with %s", shared);
     // (the stride of a single row is never taken: whatever it is, it must not decide which kernel runs)
     const long la = m > 1 ? lda : 0, lb = n > 1 ? ldb : 0;
     GemmParams p{a_dev, b_dev, a_scale_dev, b_scale_dev, la, lb, (long)ldsa, (long)ldsb, a_tile != 0, b_tile != 0, bias_dev, bias_dtype, c_dev,
@@ -218,6 +243,11 @@ int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev,
     const hipStream_t s = (hipStream_t)stream;
     with_type(c_dtype, [&](auto t) { launch_gemm<decltype(t)>(p, (float*)work_dev, work_bytes, s); });
     return ops_launched("ml_fp8_matmul");
+}
+
+int ml_debug_areas_apart(int64_t at, int64_t pitch, int64_t width, int64_t rows, int64_t at2, int64_t pitch2, int64_t width2, int64_t rows2) {
+    if ((rows > 1 && pitch < width) || (rows2 > 1 && pitch2 < width2)) return 0;
+    return apart(Area{at, pitch, width, rows}, Area{at2, pitch2, width2, rows2});
 }
 
 // ---- a linear layer in one call: buffers at multiples of 256 bytes inside two workspaces

@@ -147,7 +147,8 @@ def matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16, out=None
     results from exact bf16 operands at half the rate (4e-8; the operands' values have to lie in fp32's normal range, smaller ones count as 0).
 
     Each scale is (rows, ceil(k / 128)) or (ceil(rows / 128), ceil(k / 128)), as ``quantize`` gives them.  ``out``: an (m, n) tensor of one
-    of the three types with contiguous rows to write into (``out_dtype`` is then its type).  Not differentiable: see ``linear``."""
+    of the three types with contiguous rows to write into (``out_dtype`` is then its type), apart in memory from what is read.  Not
+    differentiable: see ``linear``."""
     index = _device_of('matmul', a, a_scale, b, b_scale, bias, out)
     if not (a.dtype == CODES and b.dtype == CODES and a.dim() == 2 and b.dim() == 2):
         raise ValueError("matmul: a and b are matrices of %s, got %s %s and %s %s" % (CODES, tuple(a.shape), a.dtype, tuple(b.shape), b.dtype))
