@@ -113,7 +113,8 @@ def quantize(x, block=(1, BLOCK), transposed=False):
 
     ``transposed=True``: (codes, scales, codes_t, scales_t) from one read of x: the same, and x^T (n, m) in blocks of ITS rows -- what a
     product needs that reduces over the other axis.  With (128, 128) blocks the transposed codes and scales are the straight ones,
-    transposed.  Rows of the codes start on 16 bytes (a view of a wider buffer where n is no multiple of 16).  Not differentiable."""
+    transposed.  Rows of the codes start on 16 bytes (a view of a wider buffer where n is no multiple of 16).  Not differentiable: x's
+    values are taken without their history."""
     _device_of('quantize', x)
     _need(x.dim() == 2 and x.dtype in DTYPES, "quantize: needs a matrix in fp32, bf16 or fp16, got %s %s", tuple(x.shape), x.dtype)
     _need(tuple(block) in ((1, BLOCK), (BLOCK, BLOCK)), "quantize: blocks are (1, 128) or (128, 128), got %r", block)
@@ -160,9 +161,9 @@ def matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16, out=None
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != n or bias.dtype not in DTYPES:
             raise ValueError("matmul: the bias is (%d) in fp32, bf16 or fp16, got %s %s" % (n, tuple(bias.shape), bias.dtype))
-        if bias.requires_grad and torch.is_grad_enabled():
-            raise ValueError("matmul is not differentiable: use linear, or detach the bias")
         bias = bias.contiguous()
+    if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad or a_scale.requires_grad or b_scale.requires_grad or (bias is not None and bias.requires_grad)):
+        raise ValueError("matmul is not differentiable: use linear, or detach the operands and the bias")
     given = out is not None
     if not given:
         if out_dtype not in DTYPES:
