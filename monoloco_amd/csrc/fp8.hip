@@ -167,6 +167,12 @@ long norm_groups(long m, long n) {
     return g < most ? g : most;
 }
 
+template <typename T>
+void launch_reduce(const float* part, long groups, long n, T* out, hipStream_t s) {
+    if (n >= 256 * 32) reduce_rows_kernel<T, 32><<<(unsigned)((n + 31) / 32), 1024, 0, s>>>(part, groups, n, out);
+    else reduce_rows_kernel<T, 16><<<(unsigned)((n + 15) / 16), 1024, 0, s>>>(part, groups, n, out);
+}
+
 // the bias gradient alone: the tile kernel without either form of codes
 int column_sums(const void* x, int dtype, int64_t m, int64_t n, int64_t ldx, float* out, hipStream_t s) {
     const int es = elem_size(dtype);
@@ -363,7 +369,7 @@ int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int
     if (n == 0) return ML_OK;
     if (!dw_dev || (m > 0 && (!dy_dev || !h_dev || !w_dev || !dx_dev || !work_dev))) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: null pointer");
     if (m > 0 && (ldy < n || ldh < n || (dh_dev && ldd < n) || ldx < n)) return ops_fail(ML_ERR_ARG, "ml_rms_norm_backward: a row stride is shorter than its row");
-    if (!fits((n + REDUCE_COLS - 1) / REDUCE_COLS, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm_backward: %lld columns are too many", (long long)n);
+    if (!fits((n + 31) / 32, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_rms_norm_backward: %lld columns are too many", (long long)n);
     const hipStream_t s = (hipStream_t)stream;
     const long groups = m ? norm_groups(m, n) : 0;
     if (m > 0) {
@@ -374,7 +380,7 @@ int ml_rms_norm_backward(const void* dy_dev, int64_t ldy, const void* h_dev, int
         const int rc = ops_launched("ml_rms_norm_backward");
         if (rc) return rc;
     }
-    with_type(w_dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + REDUCE_COLS - 1) / REDUCE_COLS), 1024, 0, s>>>(work_dev, groups, n, (decltype(t)*)dw_dev); });
+    with_type(w_dtype, [&](auto t) { launch_reduce(work_dev, groups, n, (decltype(t)*)dw_dev, s); });
     return ops_launched("ml_rms_norm_backward");
 }
 
@@ -382,8 +388,8 @@ int ml_sum_rows(const float* part_dev, int64_t rows, int64_t n, void* out_dev, i
     if (!elem_size(dtype) || rows < 0 || n < 0) return ops_fail(ML_ERR_ARG, "ml_sum_rows: bad type %d or size", dtype);
     if (n == 0) return ML_OK;
     if (!out_dev || (rows > 0 && !part_dev)) return ops_fail(ML_ERR_ARG, "ml_sum_rows: null pointer");
-    if (!fits((n + REDUCE_COLS - 1) / REDUCE_COLS, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_sum_rows: %lld columns are too many", (long long)n);
-    with_type(dtype, [&](auto t) { reduce_rows_kernel<decltype(t)><<<(unsigned)((n + REDUCE_COLS - 1) / REDUCE_COLS), 1024, 0, (hipStream_t)stream>>>(part_dev, rows, n, (decltype(t)*)out_dev); });
+    if (!fits((n + 31) / 32, 1024)) return ops_fail(ML_ERR_SHAPE, "ml_sum_rows: %lld columns are too many", (long long)n);
+    with_type(dtype, [&](auto t) { launch_reduce(part_dev, rows, n, (decltype(t)*)out_dev, (hipStream_t)stream); });
     return ops_launched("ml_sum_rows");
 }
 

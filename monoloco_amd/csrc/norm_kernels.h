@@ -261,12 +261,12 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void rms_norm_back_kerne
 }
 
 // out[c] = sum over g of part[g * n + c] in 64 bits (in 32 the join alone rounded as often as all sums before it), in a fixed order: COLS
-// columns per workgroup, 1024 / COLS teams take g = t, t + teams, ..., eight loads of each in flight.  1024 x 1024: 3.9 us (loads one after
-// the other: 11; 64-bit sums with 32 columns: 5.8, with 8: 3.1, but 12.9 instead of 4.6 for 512 x 8192; 32-bit sums: 3.6).
-constexpr int REDUCE_COLS = 16;
-template <typename T>
+// columns per workgroup, 1024 / COLS teams take g = t, t + teams, ..., eight loads of each in flight (one after the other: 11 us for 1024 x
+// 1024).  32 columns (whole 128-byte lines) where those give every CU a workgroup, else 16: 1024 x 1024 3.4 us (with 32: 5.0), 512 x 4096 2.8
+// (3.5), 512 x 8192 3.6 (with 16: 4.0).
+template <typename T, int COLS>
 __global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restrict__ part, long groups, long n, T* __restrict__ out) {
-    constexpr int COLS = REDUCE_COLS, TEAMS = 1024 / COLS;
+    constexpr int TEAMS = 1024 / COLS;
     __shared__ double s[16][COLS];
     const int cx = threadIdx.x % COLS, t = threadIdx.x / COLS;
     const long c = (long)blockIdx.x * COLS + cx;
@@ -275,7 +275,9 @@ __global__ __launch_bounds__(1024) void reduce_rows_kernel(const float* __restri
         for (long g = t; g < groups; g += 8 * TEAMS) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = g + TEAMS * u < groups ? part[(g + TEAMS * u) * n + c] : 0.0f;
+            for (int u = 0; u < 8; ++u) v[u] = part[min(g + TEAMS * u, groups - 1) * n + c];   // (no branch: hipcc would put the conversions into it)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = g + TEAMS * u < groups ? v[u] : 0.0f;
             a += (((double)v[0] + v[1]) + ((double)v[2] + v[3])) + (((double)v[4] + v[5]) + ((double)v[6] + v[7]));
         }
 #pragma unroll

@@ -7,7 +7,7 @@ from monoloco_amd import fp8
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize('rows,n', [(1, 1), (2, 5), (31, 40), (257, 33), (1024, 100), (5000, 7), (0, 9)])
+@pytest.mark.parametrize('rows,n', [(1, 1), (2, 5), (31, 40), (257, 33), (1024, 100), (5000, 7), (0, 9), (300, 8191), (300, 8192), (70, 20001)])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
 def test_sum_rows(cuda_device, hip_lib, rows, n, dtype):
     """In 64 bits, rounded once: `rows` terms of at most 53 bits each add 2^-53 rows of the magnitudes' sum to half a step of the result."""
