@@ -423,7 +423,7 @@ const char* ml_matching_last_error(void);
  * has scale 255 = NaN and NaN codes.  A block is 1 x 128 of a row (scales: (rows, ceil(cols / 128))) or 128 x 128 of a matrix ("tile":
  * (ceil(rows / 128), ceil(cols / 128))); the last block of a row may be shorter.  No counterpart in the reference, whose layers are fp32.
  * All sizes are element counts, all ld* row strides in elements; every operand's last axis is contiguous; pointers need the alignment of
- * their element only (16-byte aligned rows take wider accesses).  Asynchronous on `stream`, nothing is allocated or kept: these calls may
+ * their element only (the product runs at its full rate where the rows of both operands' codes start on 16 bytes).  Asynchronous on `stream`, nothing is allocated or kept: these calls may
  * be captured into a graph (ml_adamw_step refuses: its step number is part of the launch).  Error text: ml_ops_last_error(). */
 #define ML_F32 0
 #define ML_BF16 1
@@ -436,7 +436,7 @@ int ml_fp8_quantize(const void* x_dev, int dtype, int64_t m, int64_t n, int64_t 
                     float* colsum_dev, void* stream);
 /* c (m, n) = a (m, k) . b (n, k)^T [+ bias (n)] in fp32 accumulation, rounded once to c_dtype; a, b codes with scales per row block or
  * per tile (a_tile, b_tile).  k = 0 gives the bias (or zeros).  16-bit results come from the 8-bit matrix instructions (1.5e-5 of the result's
- * norm, far below their rounding), fp32 results from exact bf16 operands at half the rate (4e-8); there the values that the operands stand
+ * norm, far below their rounding), fp32 results from exact bf16 operands at half the rate (6e-8); there the values that the operands stand
  * for have to lie in fp32's normal range (smaller ones count as 0).  c may not share memory with what the call reads (refused). */
 int ml_fp8_matmul(const uint8_t* a_dev, int64_t lda, const uint8_t* a_scale_dev, int64_t ldsa, int a_tile, const uint8_t* b_dev, int64_t ldb,
                   const uint8_t* b_scale_dev, int64_t ldsb, int b_tile, const void* bias_dev, int bias_dtype, void* c_dev, int c_dtype,

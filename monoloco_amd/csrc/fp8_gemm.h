@@ -9,9 +9,12 @@
 //
 // Precision: measured, the 8-bit matrix instructions (scaled or not) align the products of 8 neighbouring k to the largest of them and
 // keep 13 bits below it before they reach the fp32 accumulator: 1.5e-5 of the result's norm for normal data, the same for every k.
-// That is a hundredth of bf16's rounding and a twentieth of fp16's, so results of those types use them.  fp32 results do not: there the
-// codes become bf16 in registers (exact: 4 significant bits; the scale is applied in the same conversion, exact as a power of two)
-// and v_mfma_f32_32x32x16_bf16 sums them -- half the rate, 4e-8 of the norm.
+// That is a hundredth of bf16's rounding and a twentieth of fp16's, so results of those types use them: 1.5 % of the bf16 results round to
+// the other neighbour than an fp32 product's (2.6e-4 of the norm between the two), both are 1.66e-3 from the exact result.  What it is small
+// against is the norm, not each result: where the terms cancel to less than 1e-5 of it, the 16-bit result keeps no digits.  fp32 results do
+// not use them: there the codes become bf16 in registers (exact: 4 significant bits; the scale is applied in the same conversion, exact as a
+// power of two) and v_mfma_f32_32x32x16_bf16 sums them -- half the rate, 6e-8 of the norm with the result's own rounding.  (The kernel of
+// few rows could do that for 16-bit results, too: 1 x 4096 x 4096 5.7 -> 6.3 us, 1 x 1024 x 1024 2.7 -> 3.5; left to who asks for fp32.)
 #pragma once
 #include <type_traits>
 
@@ -495,7 +498,7 @@ __device__ __forceinline__ float from_acc(float a) {
 }
 
 // ---- the streaming kernel: 256 x 256 tiles, 16-bit results, a workgroup per CU that walks tiles without a pause ----------------------
-// The ring kernel's steps with 4 x 4 matrix tiles per wave, for k a multiple of 128 from 512 on, n a multiple of 8.  There a tile of 16 steps spent 17000 of
+// The ring kernel's steps with 4 x 4 matrix tiles per wave, for k a multiple of 128, n a multiple of 8 (the launch asks for k >= 1024).  There a tile of 16 steps spent 17000 of
 // its 38000 cycles outside its products (start and addresses 5000, first latency 3600, epilogue 8000).  Here the last four steps of a tile
 // already request the first four of the next one; the next tile's scales and bias are loaded in front of the epilogue and written to LDS
 // behind it; and the epilogue needs no LDS: v_permlane32_swap joins the 4 + 4 columns of two lanes into 16 bytes of a row, stored
@@ -649,7 +652,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void f
         const int vn = v + (int)gridDim.x;
         const bool more = vn < tiles;   // (the same for the whole workgroup)
         long mn = m0, nn = n0;
-        // (a tile of 8 steps goes over to the next tile's requests behind step 3)
+        // (16 steps at least: the last four, which request the next tile's first ones, are in the loop)
         step(0, f0, f1, no, yes, none);
         step(1, f1, f0, yes, no, none);
         step(2, f0, f1, no, no, none);
@@ -679,7 +682,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void f
         __builtin_amdgcn_sched_barrier(0);
         Scales t;
         load_scales(t, mn, nn, 0);
-        // (16 columns are wholly inside or outside: n is a multiple of 8)
+        // (a lane's 8 columns are wholly inside or outside: n is a multiple of 8)
         T* const out0 = (T*)p.c + (m0 + wm * 128 + ml) * p.ldc + n0 + wn * 128 + 8 * hh;
         const int rows = (int)min(p.m - (m0 + wm * 128 + ml), 128L), cols = (int)min(p.n - (n0 + wn * 128 + 8 * hh), 128L);
         auto columns = [&](auto edge) {   // EDGE: a branch around every store

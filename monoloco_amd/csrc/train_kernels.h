@@ -1040,8 +1040,8 @@ __global__ __launch_bounds__(256) void skinny_out_kernel(const float* __restrict
         }
         __syncthreads();
         if (i0 + step < m) request(i0 + step);
-        // packed fp32 FMAs (v_pk_fma_f32: two of the same fmaf per lane and instruction -- same bits, half the VALU instructions;
-        // measured neutral at 65536 rows: the pass is bound by its store / staging latency, not by the VALU)
+        // (pairs of columns: two of the same fmaf each.  The build switches packed fp32 instructions off; with them half the VALU
+        // instructions measured neutral at 65536 rows: the pass is bound by its store / staging latency, not by the VALU)
         f32x2 alo[4] = {b4.xy, b4.xy, b4.xy, b4.xy}, ahi[4] = {b4.zw, b4.zw, b4.zw, b4.zw};
         for (int c = 0; c < nc; ++c) {
             const f32x4 wv = *(const f32x4*)&wl[c][cg * 4];
@@ -1131,7 +1131,7 @@ __global__ __launch_bounds__(256) void skinny_dw_kernel(const float* __restrict_
                     const f32x4 sv = *(const f32x4*)&ss[rg + 16 * q][c4 * 4];
 #pragma unroll
                     for (int cc = 0; cc < 4; ++cc)
-                        if (c4 * 4 + cc < NCT) {   // packed fp32 FMAs (v_pk_fma_f32): the same fmaf per element, two per instruction (neutral)
+                        if (c4 * 4 + cc < NCT) {   // (pairs of columns: the same fmaf per element; packed fp32 instructions are switched off)
                             const f32x2 s2 = {sv[cc], sv[cc]};
                             f32x2 lo = {acc[c4 * 4 + cc][0], acc[c4 * 4 + cc][1]}, hi = {acc[c4 * 4 + cc][2], acc[c4 * 4 + cc][3]};
                             lo = __builtin_elementwise_fma(s2, v[q].xy, lo);

@@ -144,8 +144,9 @@ def _matmul_work(m, n, k, dtype):
 
 def matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16, out=None):
     """a (m, k) . b (n, k)^T [+ bias (n)] of e4m3 codes with their block scales -> (m, n) in ``out_dtype`` (fp32, bf16, fp16), accumulated
-    in fp32 and rounded once.  16-bit results come from the 8-bit matrix instructions (1.5e-5 of the result's norm beside the rounding), fp32
-    results from exact bf16 operands at half the rate (4e-8; the operands' values have to lie in fp32's normal range, smaller ones count as 0).
+    in fp32 and rounded once.  16-bit results come from the 8-bit matrix instructions (1.5e-5 of the result's norm beside the rounding: a result
+    whose terms cancel to less than that keeps no digits), fp32 results from exact bf16 operands at half the rate (6e-8; the operands' values
+    have to lie in fp32's normal range, smaller ones count as 0): ``out_dtype`` is the choice between the two.
 
     Each scale is (rows, ceil(k / 128)) or (ceil(rows / 128), ceil(k / 128)), as ``quantize`` gives them.  ``out``: an (m, n) tensor of one
     of the three types with contiguous rows to write into (``out_dtype`` is then its type), apart in memory from what is read.  Not
