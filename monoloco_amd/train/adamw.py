@@ -165,7 +165,7 @@ class AdamW(torch.optim.Optimizer):
             need = {'step', 'exp_avg', 'exp_avg_sq'} | ({'scales'} if g.get('state_bits', 32) == 8 else set())
             for i in g['params']:
                 keys = set(state_dict['state'].get(i) or need)
-                _need(need <= keys <= need | {'max_exp_avg_sq'}, "AdamW: the state of another optimizer: %s", sorted(keys))
+                _need(need <= keys and 'mu_product' not in keys, "AdamW: the state of another optimizer: %s", sorted(keys))
         super().load_state_dict(state_dict)
         ids = [i for g in saved_groups for i in g['params']]
         for g, mine in zip(self.param_groups, own):
@@ -174,9 +174,9 @@ class AdamW(torch.optim.Optimizer):
         for i, p in zip(ids, [p for g in self.param_groups for p in g['params']]):
             saved = state_dict['state'].get(i)
             if saved:
-                state = {'step': int(saved['step'])}
+                state = self.state[p]      # (what a caller keeps there beside stays as the base class loaded it)
+                state['step'] = int(saved['step'])
                 for k in ('exp_avg', 'exp_avg_sq', 'scales'):
                     if k in saved:
                         v = saved[k].detach().to(p.device).clone()
                         state[k] = v.float() if v.dtype in DTYPES else v
-                self.state[p] = state

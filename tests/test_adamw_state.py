@@ -52,6 +52,16 @@ def test_states_of_the_same_rule_load():
             assert o.state[p]['step'] == 1 and all(torch.equal(o.state[p][k], saved['state'][i][k]) for k in ('exp_avg', 'exp_avg_sq'))
 
 
+def test_what_a_caller_keeps_beside_the_moments_loads():
+    a = AdamW(params())
+    for p in a.param_groups[0]['params']:
+        a._state(p, 32)['average'] = p.detach().clone() + 1
+    b = AdamW(params())
+    b.load_state_dict(copy.deepcopy(a.state_dict()))
+    for p, q in zip(a.param_groups[0]['params'], b.param_groups[0]['params']):
+        assert set(b.state[q]) == {'step', 'exp_avg', 'exp_avg_sq', 'average'} and torch.equal(b.state[q]['average'], a.state[p]['average'])
+
+
 @pytest.mark.parametrize('kw,text', [(dict(maximize=True), 'maximize'), (dict(amsgrad=True), 'amsgrad'), (dict(decoupled_weight_decay=False), 'decay'),
                                      (dict(state_bits=16), 'bits'), (dict(betas=(0.9, 1.0)), 'betas'), (dict(lr=-1.0), 'lr')])
 def test_groups_are_checked(kw, text):
